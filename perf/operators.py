@@ -242,8 +242,9 @@ def run(state):
 
 def _own_norm(st):
     from siliconed_b200 import lm_abi
-    lm_abi.rms_norm_quantize(st["x"], st["delta"], st["weight"], EPS, st["x_out"], st["codes"], st["scales"])
-    return {"x": st["x_out"] if st["delta"] is not None else st["x"], "codes": st["codes"], "scales": st["scales"]}
+    out = st["x"] if st["delta"] is None else st["x_out"]
+    lm_abi.rms_norm_quantize(st["x"], st["delta"], st["weight"], EPS, out, st["codes"], st["scales"])
+    return {"x": out, "codes": st["codes"], "scales": st["scales"]}
 
 
 def _own_append(st):
