@@ -1,10 +1,11 @@
-"""Builds the two libraries in-tree with nvcc for sm_100a (B200).
+"""Builds the three libraries in-tree with nvcc for sm_100a (B200).
 
 ``python -m siliconed_b200.build`` (or ``__graft_entry__.build()``) compiles the CUDA sources under
-``siliconed_b200/csrc`` into ``siliconed_b200/libsiliconed_cuda.so`` (the quantized linear stage) and
+``siliconed_b200/csrc`` into ``siliconed_b200/libsiliconed_cuda.so`` (the quantized linear stage),
 those under ``siliconed_b200/csrc/dit`` into ``siliconed_b200/libsiliconed_dit.so`` (the DiT blocks'
-elementwise stages).  Both link the CUDA runtime statically; the first resolves the one driver entry
-point it needs (cuTensorMapEncodeTiled) at run time, so they depend on nothing but the NVIDIA driver.
+elementwise stages) and those under ``siliconed_b200/csrc/lm`` into ``siliconed_b200/libsiliconed_lm.so``
+(the decoder layer's operators).  All link the CUDA runtime statically and resolve the one driver entry
+point they need (cuTensorMapEncodeTiled) at run time, so they depend on nothing but the NVIDIA driver.
 """
 from __future__ import annotations
 
@@ -21,6 +22,9 @@ LIB = os.path.join(HERE, "libsiliconed_cuda.so")
 DIT_LIB = os.path.join(HERE, "libsiliconed_dit.so")
 DIT_CSRC = os.path.join(CSRC, "dit")
 DIT_SOURCES = ["sd_kernels.cu", "sd_attention.cu"]
+LM_LIB = os.path.join(HERE, "libsiliconed_lm.so")
+LM_CSRC = os.path.join(CSRC, "lm")
+LM_SOURCES = ["sl_errors.cu", "sl_norm.cu", "sl_append.cu", "sl_attention.cu", "sl_linear.cu"]
 
 SOURCES = ["sc_abi.cu", "sc_weight.cu", "sc_gemm.cu", "sc_gemm_pair.cu", "sc_gemm_bf16.cu", "sc_gemm_skinny.cu", "sc_gemm_skinny_sk.cu",
            "sc_gemv.cu", "sc_no_alloc.cu", "sc_rotate.cu", "sc_w8a8.cu"]
@@ -64,6 +68,8 @@ def build(force: bool = False, verbose: bool = False) -> str:
         _compile(LIB, CSRC, SOURCES, verbose)
     if force or _stale(DIT_LIB, DIT_CSRC, "siliconed_dit.h"):
         _compile(DIT_LIB, DIT_CSRC, DIT_SOURCES, verbose)
+    if force or _stale(LM_LIB, LM_CSRC, "siliconed_lm.h"):
+        _compile(LM_LIB, LM_CSRC, LM_SOURCES, verbose)
     return LIB
 
 
