@@ -13,13 +13,25 @@
 // that it sets back to zero) adds the parts in the order of the shares, so every call gives the same bits.  A CTA
 // leaves at most two parts (its first and its last context), so the workspace does not grow with the batch.
 //
-// Inside a CTA each of the 4 warps takes tiles of 16 tokens with a maximum, sum and output of its own, joined through
-// shared memory at the context's end.  Both products run on mma.sync m16n8k16 with the cache as the A operand:
+// Inside a CTA each warp takes steps of 32 tokens with a maximum, sum and output of its own, joined through shared
+// memory at the context's end.  Both products run on mma.sync m16n8k16 with the cache as the A operand:
 // S^T = K q^T (16 tokens x 8 query heads) and O^T += V^T P^T (16 dims x 8 query heads).  The reduction index of either
-// product may be permuted freely when both operands agree, so every lane loads 16 consecutive bytes of a cache
-// row straight into the registers that the MMA reads: nothing of the cache goes through shared memory.  At one
-// query row a tcgen05 tile (128 rows) would be 94 to 99 % padding and its operands would have to be staged, rotated
-// and awaited; the MMA work here is a few percent of the tensor pipe.
+// product may be permuted freely when both operands agree, so every lane reads 16 consecutive bytes of a cache row as
+// the registers of its MMA fragments: no transposition, no ldmatrix.  At one query row a tcgen05 tile (128 rows) would
+// be 94 to 99 % padding and its operands would have to be rearranged and awaited; the MMA work here is a few percent
+// of the tensor pipe.
+//
+// The cache reaches shared memory by bulk copies (cp.async.bulk) that each warp issues for itself, two to three steps
+// ahead: token rows that follow one another in a page are one copy, whatever the page size; every lane looks up one
+// token.  (Measured on the way: 16-byte cp.async by every lane read 5.2 TB/s, bound by the 170 instructions a step
+// of addresses and copies; a copy kernel of bulk copies alone reads 6.8 TB/s in rows of 256 bytes, 4.2 in rows of 128,
+// 7.1 in runs of 16 rows.)
+//
+// An e4m3 cache runs in f16: codes are exact in it, q is first brought to a largest magnitude in [1, 2) by a power of
+// two per head, and p times its token's scale is taken relative to the largest scale so far (a second running
+// maximum), times 2^15, so that it uses f16's whole range.
+#include <cuda_fp16.h>
+
 #include <cmath>
 
 #include "sl_common.cuh"
@@ -27,11 +39,9 @@
 namespace sl {
 namespace {
 
-constexpr int kWarps = 4, kThreads = kWarps * 32;
-constexpr int kTile = 16;                 // tokens of a warp's step
-constexpr int kUnit = kWarps * kTile;     // tokens of a unit of work
-constexpr int kCtasPerSm = 2;
-constexpr int kMaxBatch = 1024;           // sequences of a launch
+constexpr int kStep = 32;                 // tokens of a warp's step: two MMA tiles of 16
+constexpr int kLeastUnits = 2;            // of a share: a cut costs more than a step
+constexpr int kMaxBatch = 512;            // sequences of a launch
 
 struct Attention {
   const uint16_t* q;
@@ -56,12 +66,19 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+template <bool kHalf>
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  if (kHalf)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 // An 8 x 8 tile of 16-bit values transposed across the warp.
@@ -71,18 +88,29 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   return r;
 }
 
-// Four e4m3 codes to bf16, exactly: the seven low bits of a code moved under bf16's exponent read as
-// value * 2^-120 (subnormal codes included), so one multiplication by 2^120 finishes it.  The cache holds no NaN
-// codes that matter: a NaN value makes its head's scale NaN.
-__device__ __forceinline__ void e4m3x4_to_bf16(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  const __nv_bfloat162 up = __nv_bfloat162(__ushort_as_bfloat16(0x7B80), __ushort_as_bfloat16(0x7B80));
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t p = __byte_perm(w, 0, i == 0 ? 0x1404 : 0x3424);  // code 2i in byte 1, code 2i + 1 in byte 3
-    const uint32_t r = ((p & 0x7F007F00u) >> 4) | (p & 0x80008000u);
-    const __nv_bfloat162 h = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&r), up);
-    (i == 0 ? lo : hi) = *reinterpret_cast<const uint32_t*>(&h);
-  }
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Four e4m3 codes to f16, exactly (NaN codes to NaN): codes 0 and 1, codes 2 and 3.
+__device__ __forceinline__ void e4m3x4_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\t"
+      "mov.b32 {a, b}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, a;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(w));
+}
+
+// An asynchronous copy of 4 bytes to shared memory, zeros where `there` is false.
+__device__ __forceinline__ void copy_async4(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
 }
 
 // The share of work: CTA w of W takes units [w T / W, (w + 1) T / W); unit u belongs to CTA ((u + 1) W - 1) / T.
@@ -91,27 +119,66 @@ __device__ __forceinline__ int64_t share_of(int64_t u, int64_t total, int64_t wo
   return ((u + 1) * workers - 1) / total;
 }
 
-// kNH: tiles of 8 query heads (1 or 2).
-template <int kDim, bool kE4m3, int kNH>
-__global__ void __launch_bounds__(kThreads, 2) paged_attention_k(const Attention a) {
-  constexpr int kRows = 8 * kNH;
-  constexpr int kBytes = kE4m3 ? 1 : 2;
-  constexpr int kRowBytes = kDim * kBytes;
-  constexpr int kKLoads = kRowBytes / 64;                 // 16-byte loads of a key row a lane: 4 lanes share a row
-  constexpr int kVWidth = kRowBytes >= 128 ? 16 : 8;      // bytes a lane loads of a value row: 8 lanes share a row
-  constexpr int kVLoads = kRowBytes / (8 * kVWidth);
-  constexpr int kVDims = kVWidth / kBytes;                // dims a lane holds of one load
-  constexpr int kPairs = kDim / 16;                       // M tiles of O^T
-  constexpr int kPartFloats = kRows * (kDim + 2);
+// Geometry of a step's 32 tokens in shared memory: rows in order.  Lane (g, c) reads bytes 64 j + 16 c .. of the key rows
+// g + 8 i, i < 4 (two lanes a bank), and kVWidth bytes at 8 e kVWidth + g kVWidth of the value rows 16 t + 2 c, + 1, + 8,
+// + 9: value rows of 256 bytes are copied one by one, 272 bytes apart, so that these reads meet no bank twice; shorter
+// ones in runs, since copies of 128 bytes are too many, at four lanes a bank (half of shared memory's rate then).
+// A warp's ring has kSlots slots that take a step's keys, its values, the next step's keys and so on.
+// kWide: one CTA an SM, for few contexts: a long context is cut into fewer parts, and more threads add them.  Else
+// CTAs of 4 warps, for many contexts: one begins while another ends.
+template <int kDim, bool kE4m3, int kNH, bool kWide>
+struct Shape {
+  static constexpr int kRows = 8 * kNH;
+  static constexpr int kRowBytes = kDim * (kE4m3 ? 1 : 2);
+  static constexpr bool kBig = kRowBytes >= 256;
+  static constexpr int kWarpsPerSm = kBig || (kNH == 2 && kDim == 128) ? 8 : 12;  // by shared memory and registers
+  static constexpr int kWarps = kWide ? kWarpsPerSm : 4;
+  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kCtasPerSm = kWarpsPerSm / kWarps;
+  static constexpr int kUnit = kWarps * kStep;                  // tokens of a unit of work
+  static constexpr int kKLoads = kRowBytes / 64;
+  static constexpr int kVWidth = kRowBytes >= 128 ? 16 : 8;
+  static constexpr int kVLoads = kRowBytes / (8 * kVWidth);
+  static constexpr int kVDims = kVWidth / (kE4m3 ? 1 : 2);
+  static constexpr int kVPitch = kBig ? kRowBytes + 16 : kRowBytes;
+  static constexpr int kSlotBytes = kStep * kVPitch;
+  static constexpr int kSlots = kBig ? 3 : kRowBytes >= 128 ? 4 : 8;
+  static constexpr int kAhead = (kSlots + 1) / 2;               // steps begun before a step is used
+  static constexpr int kScaleAt = kSlots * kSlotBytes;          // e4m3: scales of kAhead + 1 steps, 32 of k and 32 of v
+  static constexpr int kWarpBytes = kScaleAt + (kE4m3 ? (kAhead + 1) * 256 : 0);  // reused for the join
+  static constexpr int kSmem = kWarps * kWarpBytes;
+  static constexpr int kPartRow = kDim + 4;
+  static constexpr int kPartFloats = kRows * (kDim + 2);
+  static_assert(kRows * kPartRow * 4 <= kWarpBytes, "the join's part fits the ring");
+  static_assert(!kE4m3 || kSlots % 2 == 0, "the scales go with whole steps");
+};
+constexpr int kMostCtasPerSm = 3;
 
+// kNH: tiles of 8 query heads (1 or 2).
+template <int kDim, bool kE4m3, int kNH, bool kWide>
+__global__ void __launch_bounds__(Shape<kDim, kE4m3, kNH, kWide>::kThreads, Shape<kDim, kE4m3, kNH, kWide>::kCtasPerSm)
+    paged_attention_k(const Attention a) {
+  using S = Shape<kDim, kE4m3, kNH, kWide>;
+  constexpr int kWarps = S::kWarps, kThreads = S::kThreads, kUnit = S::kUnit;
+  constexpr int kRows = S::kRows, kRowBytes = S::kRowBytes, kKLoads = S::kKLoads, kVWidth = S::kVWidth;
+  constexpr int kVLoads = S::kVLoads, kVDims = S::kVDims, kSlots = S::kSlots, kAhead = S::kAhead, kVPitch = S::kVPitch, kPartFloats = S::kPartFloats;
+  constexpr int kPairs = kDim / 16;  // M tiles of O^T
+
+  extern __shared__ __align__(128) uint8_t ring[];
   __shared__ int64_t first_unit[kMaxBatch + 1];
   __shared__ int64_t scan[kWarps];
   __shared__ float part_m[kWarps][kRows], part_l[kWarps][kRows];
-  __shared__ __align__(16) float part_o[kWarps][kRows][kDim + 4];  // read 16 bytes at a time
-  __shared__ int last_flag;
+  __shared__ uint64_t arrived[kWarps][kSlots];
+  __shared__ int last_flag, abort_flag;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   sc::pdl_launch_dependents();
+  if (tid < kWarps * kSlots) sc::mbar_init(&arrived[0][0] + tid, 1);
+  if (tid == 0) abort_flag = 0;
+  sc::fence_mbar_init();
+  uint32_t fill = 0, take = 0, phases = 0;  // the warp's next slot to fill and to use, and the slots' parities
+  const uint32_t base = sc::smem_u32(ring) + warp * S::kWarpBytes;
+  const uint8_t* const mine = ring + warp * S::kWarpBytes;
   sc::pdl_wait();
 
   // Units of every sequence, summed: each thread takes a run of sequences.
@@ -155,7 +222,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attention_k(const Attention
         for (int i = tid; i < a.heads; i += kThreads) a.lse[static_cast<int64_t>(b) * a.heads + i] = -INFINITY;
     }
 
-  const int64_t workers = min(static_cast<int64_t>(gridDim.x), total);
+  const int64_t workers = max(min(static_cast<int64_t>(gridDim.x), total / kLeastUnits), min(total, int64_t(1)));
   if (blockIdx.x >= workers) return;
   const int64_t u_begin = share_start(blockIdx.x, total, workers), u_end = share_start(blockIdx.x + 1, total, workers);
 
@@ -182,6 +249,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attention_k(const Attention
 
     // q as the B operand of S^T: query head g of each tile of 8, the dims in the order of the key loads.
     uint32_t qf[kNH][kDim / 8];
+    float unit[kNH][2];  // of query heads 2 c and 2 c + 1: a score's factor, log2(e) included
 #pragma unroll
     for (int n = 0; n < kNH; ++n) {
       const bool there = n * 8 + g < rows;
@@ -193,9 +261,25 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attention_k(const Attention
         const uint4 v = there ? src[at] : make_uint4(0, 0, 0, 0);
         qf[n][4 * j] = v.x, qf[n][4 * j + 1] = v.y, qf[n][4 * j + 2] = v.z, qf[n][4 * j + 3] = v.w;
       }
+      unit[n][0] = unit[n][1] = a.scale_log2;
+      if (kE4m3) {
+        uint32_t top = 0;  // the exponent of the head's largest magnitude, in bf16's bits
+#pragma unroll
+        for (int j = 0; j < kDim / 8; ++j) top = max(top, max(qf[n][j] & 0x7F80u, (qf[n][j] >> 16) & 0x7F80u));
+        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+        const int e = min(max(static_cast<int>(top >> 7), 1), 253);  // 2^(127 - e) and 2^(e - 127) are normal
+        const float down = __uint_as_float(static_cast<uint32_t>(254 - e) << 23), up = __uint_as_float(static_cast<uint32_t>(e) << 23);
+#pragma unroll
+        for (int j = 0; j < kDim / 8; ++j)
+          qf[n][j] = pack_f16x2(__uint_as_float(qf[n][j] << 16) * down, __uint_as_float(qf[n][j] & 0xFFFF0000u) * down);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) unit[n][i] *= __shfl_sync(0xFFFFFFFFu, up, (2 * c + i) * 4);
+      }
     }
     float m[kNH][2], l[kNH][2];  // of query heads 2 c and 2 c + 1 of each tile; l is this lane's own sum
     float o[kNH][kPairs][4];
+    float vtop = 0.0f;           // e4m3: the largest scale of v so far; o is in units of vtop 2^-15
 #pragma unroll
     for (int n = 0; n < kNH; ++n) {
       m[n][0] = m[n][1] = -INFINITY;
@@ -204,109 +288,211 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attention_k(const Attention
       for (int i = 0; i < kPairs; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.0f;
     }
 
-    for (int t0 = t_begin + warp * kTile; t0 < t_end; t0 += kUnit) {
-      // The cache row of token t0 + (lane & 15), all ones where there is none.
-      uint32_t row = 0xFFFFFFFFu;
-      {
-        const int t = t0 + (lane & 15);
-        if (t < t_end) {
-          const int index = a.page_shift >= 0 ? t >> a.page_shift : t / a.page_size;
-          const int page = table[index];
-          if (page < 0 || page >= a.pages)
-            sc::record_error(a.err, kErrRange, kSiteAttentionPage);
-          else
-            row = (static_cast<uint32_t>(page) * a.kv_heads + kvh) * a.page_size + (t - index * a.page_size);
-        }
+    // The page of token t + lane (-1: none), asked for one step before it is used, and its cache row, all ones where
+    // there is none.
+    auto page_of = [&](int t) -> int {
+      t += lane;
+      return t < t_end ? table[a.page_shift >= 0 ? t >> a.page_shift : t / a.page_size] : -1;
+    };
+    auto row_of = [&](int t, int page) -> uint32_t {
+      t += lane;
+      if (t >= t_end) return 0xFFFFFFFFu;
+      if (page < 0 || page >= a.pages) {
+        sc::record_error(a.err, kErrRange, kSiteAttentionPage);
+        return 0xFFFFFFFFu;
       }
-      uint32_t kr[2], vr[4];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) kr[i] = __shfl_sync(0xFFFFFFFFu, row, g + 8 * i);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) vr[i] = __shfl_sync(0xFFFFFFFFu, row, 2 * c + (i & 1) + 8 * (i >> 1));
-      uint4 kd[2][kKLoads];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const char*>(a.k_cache) +
-                                                          static_cast<uint64_t>(kr[i]) * kRowBytes) + c;
-#pragma unroll
-        for (int j = 0; j < kKLoads; ++j)
-          kd[i][j] = kr[i] != 0xFFFFFFFFu ? __ldcs(src + 4 * j) : make_uint4(0, 0, 0, 0);
+      return (static_cast<uint32_t>(page) * a.kv_heads + kvh) * a.page_size +
+             (a.page_shift >= 0 ? t & (a.page_size - 1) : t % a.page_size);
+    };
+    // The tokens of a step, one a lane: its cache row, whether there is one (`there` is the mask of all lanes), and the
+    // count of rows that follow one another in the cache from here on (0 inside such a run).
+    struct Tokens {
+      uint32_t row, there;
+      int run;
+    };
+    auto tokens_of = [&](int t, int page) {
+      Tokens k;
+      const bool there = t + lane < t_end && page >= 0 && page < a.pages;
+      if (t + lane < t_end && !there) sc::record_error(a.err, kErrRange, kSiteAttentionPage);
+      k.row = (static_cast<uint32_t>(page) * a.kv_heads + kvh) * a.page_size +
+              (a.page_shift >= 0 ? (t + lane) & (a.page_size - 1) : (t + lane) % a.page_size);
+      k.there = __ballot_sync(0xFFFFFFFFu, there);
+      const uint32_t before = __shfl_up_sync(0xFFFFFFFFu, k.row, 1);
+      const bool starts = there && (lane == 0 || !((k.there >> (lane - 1)) & 1) || before + 1 != k.row);
+      const uint32_t ends = (__ballot_sync(0xFFFFFFFFu, starts) | ~k.there) & (0xFFFFFFFEu << lane);
+      k.run = starts ? (ends != 0 ? __ffs(ends) - 1 : 32) - lane : 0;
+      return k;
+    };
+    // The keys (values) of a step on their way into the next slot.
+    auto next_slot = [&](const Tokens& k) {
+      uint64_t* bar = &arrived[warp][fill];
+      if (lane == 0) sc::mbar_arrive_expect_tx(bar, __popc(k.there) * kRowBytes);
+      __syncwarp();
+      return bar;
+    };
+    auto copy = [&](uint32_t dst, const void* cache, uint32_t row, int count, uint64_t* bar) {
+      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                   "l"(static_cast<const char*>(cache) + static_cast<uint64_t>(row) * kRowBytes), "r"(count * kRowBytes),
+                   "r"(sc::smem_u32(bar))
+                   : "memory");
+    };
+    auto fetch_keys = [&](const Tokens& k) {
+      uint64_t* bar = next_slot(k);
+      if (k.run != 0) copy(base + fill * S::kSlotBytes + lane * kRowBytes, a.k_cache, k.row, k.run, bar);
+      fill = fill + 1 == kSlots ? 0 : fill + 1;
+    };
+    auto fetch_values = [&](const Tokens& k) {
+      uint64_t* bar = next_slot(k);
+      const uint32_t dst = base + fill * S::kSlotBytes + lane * kVPitch;
+      if (S::kBig ? (k.there >> lane) & 1 : k.run != 0) copy(dst, a.v_cache, k.row, S::kBig ? 1 : k.run, bar);
+      if (!((k.there >> lane) & 1)) {  // zeros where there is no token: p is 0 there, and 0 times anything finite is 0
+        for (int i = 0; i < kRowBytes; i += 16)
+          asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(dst + i), "r"(0) : "memory");
+        sc::fence_async_shared();  // before a later copy into the slot
       }
-      uint32_t vd[4][kVLoads][kVWidth / 4];
+      fill = fill + 1 == kSlots ? 0 : fill + 1;
+    };
+    // The oldest copy not yet used; null when it did not arrive in time.
+    auto arrival = [&]() -> const uint8_t* {
+      const bool ok = sc::mbar_wait(&arrived[warp][take], (phases >> take) & 1, &abort_flag, a.err, kSiteAttentionCopy);
+      const uint8_t* at = mine + take * S::kSlotBytes;
+      phases ^= 1u << take;
+      take = take + 1 == kSlots ? 0 : take + 1;
+      return __all_sync(0xFFFFFFFFu, ok) ? at : nullptr;
+    };
+
+    // Copy n is the keys of step n / 2 (n even) or its values (n odd); copy n + kSlots goes out when copy n has been used.
+    // With an odd count of slots a step's keys go out before the values of the step before them.  Pages are looked up
+    // one step before the copies need them.
+    const int t_first = t_begin + warp * kStep;
+    uint32_t masks[kAhead + 1];  // of the tokens that are there, this step's first
+    Tokens held = {0, 0, 0};
+    int page = page_of(t_first), scale_slot = 0;
+    auto fetch_scales = [&](const Tokens& k) {
+      if (kE4m3) {
+        const bool there = (k.there >> lane) & 1;
+        const uint32_t dst = base + S::kScaleAt + scale_slot * 256 + lane * 4;
+        copy_async4(dst, a.k_scale + (there ? k.row : 0), there);
+        copy_async4(dst + 128, a.v_scale + (there ? k.row : 0), there);
+        copy_commit();
+        scale_slot = scale_slot == kAhead ? 0 : scale_slot + 1;
+      }
+    };
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const char* src = static_cast<const char*>(a.v_cache) + static_cast<uint64_t>(vr[i]) * kRowBytes + g * kVWidth;
+    for (int i = 0; i < kAhead; ++i) {
+      const int t = t_first + i * kUnit, next = page_of(t + kUnit);
+      held = tokens_of(t, page);
+      masks[i] = held.there;
+      if (t < t_end) fetch_keys(held);
+      if (t < t_end && 2 * i + 1 < kSlots) fetch_values(held);
+      fetch_scales(held);
+      page = next;
+    }
+#pragma unroll 1
+    for (int t0 = t_first; t0 < t_end; t0 += kUnit) {
+      // The tokens of the step kAhead on: looked at here, or with an odd count of slots once the values are used.
+      const int t_ahead = t0 + kAhead * kUnit;
+      auto look_ahead = [&]() {
+        const int next = page_of(t_ahead + kUnit);
+        held = tokens_of(t_ahead, page);
+        masks[kAhead] = held.there;
+        fetch_scales(held);
+        page = next;
+      };
+      if (kSlots % 2 == 0) look_ahead();
+
+      float ks[4], vs[4];  // of tokens g + 8 i
+      if (kE4m3) {
+        copy_wait<kAhead>();
+        __syncwarp();  // the scales were copied by other lanes
+        const float* sc = reinterpret_cast<const float*>(mine + S::kScaleAt + scale_slot * 256);  // the slot to be filled next
 #pragma unroll
-        for (int e = 0; e < kVLoads; ++e) {
-          if (kVWidth == 16) {
-            const uint4 v = vr[i] != 0xFFFFFFFFu ? __ldcs(reinterpret_cast<const uint4*>(src + e * 128)) : make_uint4(0, 0, 0, 0);
-            vd[i][e][0] = v.x, vd[i][e][1] = v.y, vd[i][e][kVWidth / 4 - 2] = v.z, vd[i][e][kVWidth / 4 - 1] = v.w;
+        for (int i = 0; i < 4; ++i) ks[i] = sc[g + 8 * i], vs[i] = sc[32 + g + 8 * i];
+      }
+      const uint8_t* const keys = arrival();
+      if (keys == nullptr) break;
+      // S^T: tokens g + 8 i by query heads 2 c and 2 c + 1, in two MMA tiles.
+      float s[kNH][2][4];
+#pragma unroll
+      for (int n = 0; n < kNH; ++n)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) s[n][t][0] = s[n][t][1] = s[n][t][2] = s[n][t][3] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < kKLoads; ++j)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const uint8_t* at = keys + (16 * t + g) * kRowBytes + j * 64 + c * 16;
+          const uint4 k0 = *reinterpret_cast<const uint4*>(at);
+          const uint4 k1 = *reinterpret_cast<const uint4*>(at + 8 * kRowBytes);
+          const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+          if (kE4m3) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t a0, a1, a2, a3;
+              e4m3x4_to_f16(w0[i], a0, a2);
+              e4m3x4_to_f16(w1[i], a1, a3);
+#pragma unroll
+              for (int n = 0; n < kNH; ++n)
+                mma16816<true>(s[n][t], a0, a1, a2, a3, qf[n][8 * j + 2 * i], qf[n][8 * j + 2 * i + 1]);
+            }
           } else {
-            const uint2 v = vr[i] != 0xFFFFFFFFu ? __ldcs(reinterpret_cast<const uint2*>(src + e * 64)) : make_uint2(0, 0);
-            vd[i][e][0] = v.x, vd[i][e][1] = v.y;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int n = 0; n < kNH; ++n)
+                mma16816<false>(s[n][t], w0[2 * i], w1[2 * i], w0[2 * i + 1], w1[2 * i + 1], qf[n][4 * j + 2 * i],
+                                qf[n][4 * j + 2 * i + 1]);
           }
         }
-      }
-      float ks[2] = {1.0f, 1.0f}, vs[2] = {1.0f, 1.0f};  // of tokens g and g + 8
-      if (kE4m3) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          ks[i] = kr[i] != 0xFFFFFFFFu ? a.k_scale[kr[i]] : 0.0f;
-          vs[i] = kr[i] != 0xFFFFFFFFu ? a.v_scale[kr[i]] : 0.0f;
-        }
+      __syncwarp();  // the keys' slot has been read
+      if (kSlots % 2 == 0) {
+        if (t_ahead < t_end) fetch_keys(held);
+      } else {
+        if (t_ahead - kUnit < t_end) fetch_values(held);
       }
 
-      // S^T: tokens g and g + 8 by query heads 2 c and 2 c + 1.
-      float s[kNH][4];
+      float vturn = 1.0f;  // e4m3: the factor of what o summed under a smaller vtop
+      if (kE4m3) {
+        float top = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
 #pragma unroll
-      for (int n = 0; n < kNH; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
-#pragma unroll
-      for (int j = 0; j < kKLoads; ++j) {
-        const uint32_t w0[4] = {kd[0][j].x, kd[0][j].y, kd[0][j].z, kd[0][j].w};
-        const uint32_t w1[4] = {kd[1][j].x, kd[1][j].y, kd[1][j].z, kd[1][j].w};
-        if (kE4m3) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t a0, a1, a2, a3;
-            e4m3x4_to_bf16(w0[i], a0, a2);
-            e4m3x4_to_bf16(w1[i], a1, a3);
-#pragma unroll
-            for (int n = 0; n < kNH; ++n) mma16816(s[n], a0, a1, a2, a3, qf[n][8 * j + 2 * i], qf[n][8 * j + 2 * i + 1]);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int n = 0; n < kNH; ++n)
-              mma16816(s[n], w0[2 * i], w1[2 * i], w0[2 * i + 1], w1[2 * i + 1], qf[n][4 * j + 2 * i],
-                       qf[n][4 * j + 2 * i + 1]);
+        for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
+        if (top > vtop) {
+          vturn = fmaxf(vtop, 7.9e-31f) / fmaxf(top, 7.9e-31f);
+          vtop = top;
         }
+        // a floor keeps the factor finite; scales below it (smaller than any that the append writes) stay exact enough
+        const float f = 32768.0f / fmaxf(vtop, 7.9e-31f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) vs[i] *= f;
       }
-      uint32_t p[kNH][2];  // P^T as the B operand: head g, tokens 2 c, 2 c + 1 and 2 c + 8, 2 c + 9
-      const bool there0 = kr[0] != 0xFFFFFFFFu, there1 = kr[1] != 0xFFFFFFFFu;
+      uint32_t p[kNH][2][2];  // P^T as the B operand: head g, tokens 2 c, 2 c + 1 and 2 c + 8, 2 c + 9 of each tile
 #pragma unroll
       for (int n = 0; n < kNH; ++n) {
-        float x[4];
+        float x[8];  // tokens g + 8 (i >> 1), query head 2 c + (i & 1)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          x[i] = (i < 2 ? there0 : there1) ? s[n][i] * (kE4m3 ? ks[i >> 1] * a.scale_log2 : a.scale_log2) : -INFINITY;
-        float top[2] = {fmaxf(x[0], x[2]), fmaxf(x[1], x[3])};
+        for (int i = 0; i < 8; ++i)
+          x[i] = (masks[0] >> (g + 8 * (i >> 1))) & 1 ? s[n][i >> 2][i & 3] * (kE4m3 ? ks[i >> 1] * unit[n][i & 1] : unit[n][i & 1])
+                                                      : -INFINITY;
+        float top[2], zero[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) top[i] = fmaxf(fmaxf(x[i], x[2 + i]), fmaxf(x[4 + i], x[6 + i]));
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) {
           top[0] = fmaxf(top[0], __shfl_xor_sync(0xFFFFFFFFu, top[0], off));
           top[1] = fmaxf(top[1], __shfl_xor_sync(0xFFFFFFFFu, top[1], off));
         }
-        float base[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const float now = fmaxf(m[n][i], top[i]);
-          base[i] = now == -INFINITY ? 0.0f : now;  // nothing but -inf so far: every p is 0
-          top[i] = ex2(m[n][i] - base[i]);          // the factor of what was summed before
+          zero[i] = now == -INFINITY ? 0.0f : now;  // nothing but -inf so far: every p is 0
+          top[i] = ex2(m[n][i] - zero[i]);          // the factor of what was summed before
           m[n][i] = now;
         }
-        if (__any_sync(0xFFFFFFFFu, top[0] != 1.0f || top[1] != 1.0f)) {
+        if (__any_sync(0xFFFFFFFFu, top[0] != 1.0f || top[1] != 1.0f || vturn != 1.0f)) {
           l[n][0] *= top[0];
           l[n][1] *= top[1];
+          top[0] *= vturn;
+          top[1] *= vturn;
 #pragma unroll
           for (int i = 0; i < kPairs; ++i) {
             o[n][i][0] *= top[0];
@@ -316,42 +502,76 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attention_k(const Attention
           }
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = ex2(x[i] - base[i & 1]);
-        l[n][0] += x[0] + x[2];
-        l[n][1] += x[1] + x[3];
+        for (int i = 0; i < 8; ++i) x[i] = ex2(x[i] - zero[i & 1]);
+        l[n][0] += (x[0] + x[2]) + (x[4] + x[6]);
+        l[n][1] += (x[1] + x[3]) + (x[5] + x[7]);
         // The one rounding to 16 bits: p (times its token's scale of v) as the MMA's operand.
-        p[n][0] = transpose8x8(pack_bf16x2(x[0] * vs[0], x[1] * vs[0]));
-        p[n][1] = transpose8x8(pack_bf16x2(x[2] * vs[1], x[3] * vs[1]));
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          p[n][i >> 1][i & 1] = transpose8x8(kE4m3 ? pack_f16x2(x[2 * i] * vs[i], x[2 * i + 1] * vs[i])
+                                                   : pack_bf16x2(x[2 * i], x[2 * i + 1]));
       }
+      const uint8_t* const values = arrival();
+      if (values == nullptr) break;
       // O^T += V^T P^T.  M tile i of load e: rows g are dims (8 e + g) kVDims + 2 i, rows g + 8 the dims after them.
 #pragma unroll
-      for (int e = 0; e < kVLoads; ++e)
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int w = 0; w < kVWidth / 4; ++w) {
-          if (kE4m3) {
-            uint32_t lo4[4], hi4[4];
+        for (int e = 0; e < kVLoads; ++e) {
+          uint32_t v[4][kVWidth / 4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) e4m3x4_to_bf16(vd[i][e][w], lo4[i], hi4[i]);
+          for (int i = 0; i < 4; ++i) {
+            const uint8_t* src = values + (16 * t + 2 * c + (i & 1) + 8 * (i >> 1)) * kVPitch + (8 * e + g) * kVWidth;
+            if (kVWidth == 16) {
+              const uint4 u = *reinterpret_cast<const uint4*>(src);
+              v[i][0] = u.x, v[i][1] = u.y, v[i][kVWidth / 4 - 2] = u.z, v[i][kVWidth / 4 - 1] = u.w;
+            } else {
+              const uint2 u = *reinterpret_cast<const uint2*>(src);
+              v[i][0] = u.x, v[i][1] = u.y;
+            }
+          }
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const uint32_t* r = half == 0 ? lo4 : hi4;
-              const uint32_t a0 = __byte_perm(r[0], r[1], 0x5410), a1 = __byte_perm(r[0], r[1], 0x7632);
-              const uint32_t a2 = __byte_perm(r[2], r[3], 0x5410), a3 = __byte_perm(r[2], r[3], 0x7632);
+          for (int w = 0; w < kVWidth / 4; ++w) {
+            if (kE4m3) {
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                uint32_t a0, a1, a2, a3;  // the codes of two tokens side by side, dim by dim
+                e4m3x4_to_f16(__byte_perm(v[0][w], v[1][w], half == 0 ? 0x5140 : 0x7362), a0, a1);
+                e4m3x4_to_f16(__byte_perm(v[2][w], v[3][w], half == 0 ? 0x5140 : 0x7362), a2, a3);
+#pragma unroll
+                for (int n = 0; n < kNH; ++n)
+                  mma16816<true>(o[n][e * (kVDims / 2) + 2 * w + half], a0, a1, a2, a3, p[n][t][0], p[n][t][1]);
+              }
+            } else {
+              const uint32_t a0 = __byte_perm(v[0][w], v[1][w], 0x5410), a1 = __byte_perm(v[0][w], v[1][w], 0x7632);
+              const uint32_t a2 = __byte_perm(v[2][w], v[3][w], 0x5410), a3 = __byte_perm(v[2][w], v[3][w], 0x7632);
 #pragma unroll
               for (int n = 0; n < kNH; ++n)
-                mma16816(o[n][e * (kVDims / 2) + 2 * w + half], a0, a1, a2, a3, p[n][0], p[n][1]);
+                mma16816<false>(o[n][e * (kVDims / 2) + w], a0, a1, a2, a3, p[n][t][0], p[n][t][1]);
             }
-          } else {
-            const uint32_t a0 = __byte_perm(vd[0][e][w], vd[1][e][w], 0x5410), a1 = __byte_perm(vd[0][e][w], vd[1][e][w], 0x7632);
-            const uint32_t a2 = __byte_perm(vd[2][e][w], vd[3][e][w], 0x5410), a3 = __byte_perm(vd[2][e][w], vd[3][e][w], 0x7632);
-#pragma unroll
-            for (int n = 0; n < kNH; ++n) mma16816(o[n][e * (kVDims / 2) + w], a0, a1, a2, a3, p[n][0], p[n][1]);
           }
         }
+      __syncwarp();  // the values' slot has been read
+      if (kSlots % 2 == 0) {
+        if (t_ahead < t_end) fetch_values(held);
+      } else {
+        look_ahead();
+        if (t_ahead < t_end) fetch_keys(held);
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) masks[i] = masks[i + 1];
+    }
+    if (kE4m3) copy_wait<0>();
+    while (take != fill) {  // only after a wait that gave up: the copies still on their way
+      sc::mbar_wait_drain(&arrived[warp][take], (phases >> take) & 1);
+      phases ^= 1u << take;
+      take = take + 1 == kSlots ? 0 : take + 1;
     }
 
-    // Join the warps.
-    __syncthreads();  // the arrays are free (an earlier context's readers are done)
+    // Join the warps.  Each writes its part over its own ring, whose copies have all arrived.
+    const float back = kE4m3 ? fmaxf(vtop, 7.9e-31f) * (1.0f / 32768.0f) : 1.0f;
+    float* const part_o = reinterpret_cast<float*>(ring + warp * S::kWarpBytes);
+    __syncwarp();
 #pragma unroll
     for (int n = 0; n < kNH; ++n)
 #pragma unroll
@@ -367,28 +587,27 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attention_k(const Attention
 #pragma unroll
           for (int w = 0; w < kVDims / 2; ++w) {
             const float* acc = o[n][e * (kVDims / 2) + w];
-            float* dst = &part_o[warp][n * 8 + 2 * c + i][(8 * e + g) * kVDims + 2 * w];
-            *reinterpret_cast<float2*>(dst) = make_float2(acc[i], acc[2 + i]);
+            *reinterpret_cast<float2*>(part_o + (n * 8 + 2 * c + i) * S::kPartRow + (8 * e + g) * kVDims + 2 * w) =
+                make_float2(acc[i] * back, acc[2 + i] * back);
           }
       }
     __syncthreads();
     const bool whole = u == s0 && stop == s1;
     // Every thread: a run of 4 dims of the rows r0, r0 + step, ...
-    constexpr int kRun = kDim / 4, kStep = kThreads / kRun > 0 ? kThreads / kRun : 1;
-    const int slot = u == u_begin ? 0 : 1;
-    float* part = a.parts + (static_cast<int64_t>(blockIdx.x) * 2 + slot) * kPartFloats;
-    for (int r = tid / kRun; r < rows; r += kStep) {
+    constexpr int kRun = kDim / 4, kRowStep = kThreads / kRun;
+    float* part = a.parts + (static_cast<int64_t>(blockIdx.x) * 2 + (u == u_begin ? 0 : 1)) * kPartFloats;
+    for (int r = tid / kRun; r < rows; r += kRowStep) {
       const int d0 = (tid % kRun) * 4;
       float top = part_m[0][r];
 #pragma unroll
       for (int w = 1; w < kWarps; ++w) top = fmaxf(top, part_m[w][r]);
-      const float base = top == -INFINITY ? 0.0f : top;
+      const float zero = top == -INFINITY ? 0.0f : top;
       float sum = 0.0f;
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float f = ex2(part_m[w][r] - base);
-        const float4 v = *reinterpret_cast<const float4*>(&part_o[w][r][d0]);
+        const float f = ex2(part_m[w][r] - zero);
+        const float4 v = *reinterpret_cast<const float4*>(ring + w * S::kWarpBytes + (r * S::kPartRow + d0) * 4);
         sum += f * part_l[w][r];
         acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
       }
@@ -397,7 +616,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attention_k(const Attention
         const int64_t head = static_cast<int64_t>(b) * a.heads + head0 + r;
         *reinterpret_cast<uint2*>(a.out + head * kDim + d0) =
             make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
-        if (d0 == 0 && a.lse != nullptr) a.lse[head] = sum == 0.0f ? -INFINITY : (base + log2f(sum)) * 0.6931471805599453f;
+        if (d0 == 0 && a.lse != nullptr) a.lse[head] = sum == 0.0f ? -INFINITY : (zero + log2f(sum)) * 0.6931471805599453f;
       } else {
         *reinterpret_cast<float4*>(part + r * kDim + d0) = acc;
         if (d0 == 0) *reinterpret_cast<float2*>(part + kRows * kDim + 2 * r) = make_float2(top, sum);
@@ -406,9 +625,9 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attention_k(const Attention
     if (!whole) {
       // The last of the context's CTAs adds the parts, in the order of the shares.
       const int64_t wa = share_of(s0, total, workers), wb = share_of(s1 - 1, total, workers);
-      __threadfence();
       __syncthreads();
       if (tid == 0) {
+        __threadfence();  // after the barrier: the whole CTA's part
         const uint32_t before = atomicAdd(a.counters + wa, 1u);
         last_flag = before == static_cast<uint32_t>(wb - wa);
         if (last_flag) a.counters[wa] = 0u;
@@ -416,43 +635,99 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attention_k(const Attention
       }
       __syncthreads();
       if (last_flag) {
-        for (int r = tid / kRun; r < rows; r += kStep) {
-          const int d0 = (tid % kRun) * 4;
-          float top = -INFINITY, sum = 0.0f;
-          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int64_t w = wa; w <= wb; ++w) {
-            const float* src = a.parts + (w * 2 + (share_start(w, total, workers) < s0 ? 1 : 0)) * kPartFloats;
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + kRows * kDim + 2 * r));
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(src + r * kDim + d0));
-            const float now = fmaxf(top, ml.x), base = now == -INFINITY ? 0.0f : now;
-            const float f0 = ex2(top - base), f1 = ex2(ml.x - base);
-            sum = sum * f0 + ml.y * f1;
-            acc.x = acc.x * f0 + v.x * f1, acc.y = acc.y * f0 + v.y * f1;
-            acc.z = acc.z * f0 + v.z * f1, acc.w = acc.w * f0 + v.w * f1;
-            top = now;
+        // Part w lies in slot 0, but for the first one when that CTA began an earlier context.
+        const int count = static_cast<int>(wb - wa) + 1;
+        const float* first = a.parts + (wa * 2 + (share_start(wa, total, workers) < s0 ? 1 : 0)) * kPartFloats;
+        const float* others = a.parts + wa * 2 * kPartFloats;
+        auto part_of = [&](int w) { return w == 0 ? first : others + static_cast<int64_t>(w) * 2 * kPartFloats; };
+        const int d0 = (tid % kRun) * 4;
+        // The first parts' sums are on their way while every part's factor exp(m_w - m) is formed.
+        constexpr int kEarly = 4;
+        float4 early[kEarly];
+#pragma unroll
+        for (int w = 0; w < kEarly; ++w)
+          if (w < count && tid / kRun < rows) early[w] = __ldcg(reinterpret_cast<const float4*>(part_of(w) + tid / kRun * kDim + d0));
+        float2* factor = reinterpret_cast<float2*>(ring);  // [rows][count]: m, then exp(m - top), and l
+        for (int r = warp; r < rows; r += kWarps) {
+          float top = -INFINITY;
+          for (int w = lane; w < count; w += 32) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(part_of(w) + kRows * kDim + 2 * r));
+            factor[r * count + w] = ml;
+            top = fmaxf(top, ml.x);
           }
-          const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+          for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
+          const float zero = top == -INFINITY ? 0.0f : top;
+          float sum = 0.0f;
+          for (int w = lane; w < count; w += 32) {
+            const float2 ml = factor[r * count + w];
+            const float f = ex2(ml.x - zero);
+            factor[r * count + w].x = f;
+            sum += f * ml.y;
+          }
+#pragma unroll
+          for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, off);
+          if (lane == 0) {
+            part_l[0][r] = sum;
+            part_m[0][r] = zero;
+          }
+        }
+        __syncthreads();
+        for (int r = tid / kRun; r < rows; r += kRowStep) {
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+          const auto add = [&](float4 v, int w) {
+            const float f = factor[r * count + w].x;
+            acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
+          };
+          if (r == tid / kRun) {
+#pragma unroll
+            for (int w = 0; w < kEarly; ++w)
+              if (w < count) add(early[w], w);
+          } else {
+            for (int w = 0; w < min(kEarly, count); ++w) add(__ldcg(reinterpret_cast<const float4*>(part_of(w) + r * kDim + d0)), w);
+          }
+#pragma unroll 8
+          for (int w = kEarly; w < count; ++w)
+            add(__ldcg(reinterpret_cast<const float4*>(others + static_cast<int64_t>(w) * 2 * kPartFloats + r * kDim + d0)), w);
+          const float sum = part_l[0][r], inv = sum == 0.0f ? 0.0f : 1.0f / sum;
           const int64_t head = static_cast<int64_t>(b) * a.heads + head0 + r;
           *reinterpret_cast<uint2*>(a.out + head * kDim + d0) =
               make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
-          if (d0 == 0 && a.lse != nullptr) a.lse[head] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+          if (d0 == 0 && a.lse != nullptr)
+            a.lse[head] = sum == 0.0f ? -INFINITY : (part_m[0][r] + log2f(sum)) * 0.6931471805599453f;
         }
       }
     }
+    sc::fence_async_shared();
+    __syncthreads();  // the parts are read before the next context's tiles arrive
     u = stop;
   }
 }
 
-template <int kDim, bool kE4m3, int kNH>
-cudaError_t launch_attention(const Attention& a, int workers, cudaStream_t stream) {
-  return launch(paged_attention_k<kDim, kE4m3, kNH>, dim3(static_cast<unsigned>(workers)), dim3(kThreads), 0, stream, a);
+template <int kDim, bool kE4m3, int kNH, bool kWide>
+cudaError_t launch_attention(const Attention& a, int sms, cudaStream_t stream) {
+  using S = Shape<kDim, kE4m3, kNH, kWide>;
+  auto kernel = paged_attention_k<kDim, kE4m3, kNH, kWide>;
+  static unsigned long long configured = 0;
+  if (const cudaError_t e = set_smem_once(kernel, S::kSmem, configured); e != cudaSuccess) return e;
+  return launch(kernel, dim3(static_cast<unsigned>(sms * S::kCtasPerSm)), dim3(S::kThreads), S::kSmem, stream, a);
+}
+
+template <int kDim, bool kE4m3>
+cudaError_t launch_kind(const Attention& a, int sms, cudaStream_t stream) {
+  // Four-warp CTAs cut a long context into so many parts (444 over few contexts) that adding them costs more than the
+  // switches between contexts that they hide: 4 contexts of 131072 tokens 87 us, wide 68; but 8 of 16 tokens 4.9, wide
+  // 7.7, and 2048 of 128 tokens 42 either way (B200, heads of 128).
+  const bool wide = static_cast<int64_t>(a.batch) * a.kv_heads * a.subs < 64 &&
+                    static_cast<int64_t>(a.table_width) * a.page_size > 2048;
+  if (a.group <= 8)
+    return wide ? launch_attention<kDim, kE4m3, 1, true>(a, sms, stream) : launch_attention<kDim, kE4m3, 1, false>(a, sms, stream);
+  return wide ? launch_attention<kDim, kE4m3, 2, true>(a, sms, stream) : launch_attention<kDim, kE4m3, 2, false>(a, sms, stream);
 }
 
 template <int kDim>
-cudaError_t launch_dim(const Attention& a, bool e4m3, int workers, cudaStream_t stream) {
-  if (a.group <= 8)
-    return e4m3 ? launch_attention<kDim, true, 1>(a, workers, stream) : launch_attention<kDim, false, 1>(a, workers, stream);
-  return e4m3 ? launch_attention<kDim, true, 2>(a, workers, stream) : launch_attention<kDim, false, 2>(a, workers, stream);
+cudaError_t launch_dim(const Attention& a, bool e4m3, int sms, cudaStream_t stream) {
+  return e4m3 ? launch_kind<kDim, true>(a, sms, stream) : launch_kind<kDim, false>(a, sms, stream);
 }
 
 // The SMs of the current device (0: none).
@@ -483,7 +758,7 @@ extern "C" int sl_paged_attention_workspace(int heads, int kv_heads, int head_di
   if (bytes == nullptr || !shape_ok(heads, kv_heads, head_dim)) return SL_INVALID_ARG;
   const int sms = sm_count();
   if (sms == 0) return SL_CUDA_ERROR;
-  const int workers = sms * kCtasPerSm;
+  const int workers = sms * kMostCtasPerSm;
   *bytes = counter_bytes(workers) +
            static_cast<size_t>(workers) * 2 * tile_rows(heads, kv_heads) * (head_dim + 2) * sizeof(float);
   return SL_OK;
@@ -500,7 +775,7 @@ extern "C" int sl_paged_attention(const uint16_t* q, const void* k_cache, const 
     return SL_INVALID_ARG;
   // Cache rows and a sequence's tokens are counted in 32 bits.
   if (pages > 0x7FFFFFFF || static_cast<double>(pages) * kv_heads * page_size >= 4294967295.0 ||
-      static_cast<int64_t>(table_width) * page_size > 0x7FFFFFC0)
+      static_cast<int64_t>(table_width) * page_size > 0x7FFF0000)
     return SL_INVALID_ARG;
   if (batch == 0) return SL_OK;
   for (const void* p : {static_cast<const void*>(q), k_cache, v_cache, static_cast<const void*>(out),
@@ -514,7 +789,7 @@ extern "C" int sl_paged_attention(const uint16_t* q, const void* k_cache, const 
   size_t need = 0;
   if (const int s = sl_paged_attention_workspace(heads, kv_heads, head_dim, &need); s != SL_OK) return s;
   if (workspace_bytes < need) return SL_INVALID_ARG;
-  const int workers = sm_count() * kCtasPerSm;
+  const int sms = sm_count(), workers = sms * kMostCtasPerSm;
   int* err = error_word();
   if (err == nullptr) return SL_CUDA_ERROR;
   const int group = heads / kv_heads;
@@ -547,8 +822,8 @@ extern "C" int sl_paged_attention(const uint16_t* q, const void* k_cache, const 
                       reinterpret_cast<float*>(static_cast<char*>(workspace) + counter_bytes(workers)),
                       err};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const cudaError_t e = head_dim == 64 ? launch_dim<64>(a, e4m3, workers, st)
-                                         : launch_dim<128>(a, e4m3, workers, st);
+    const cudaError_t e = head_dim == 64 ? launch_dim<64>(a, e4m3, sms, st)
+                                         : launch_dim<128>(a, e4m3, sms, st);
     if (e != cudaSuccess) return status_of(e);
   }
   return SL_OK;

@@ -22,6 +22,7 @@ enum Site : int {
   kSiteAppendPage = 43,
   kSiteAttentionLength = 44,
   kSiteAttentionPage = 45,
+  kSiteAttentionCopy = 50,
   kSiteLinearLoad = 46,
   kSiteLinearMma = 47,
   kSiteLinearBuffer = 48,
@@ -41,6 +42,19 @@ inline int status_of(cudaError_t e) {
 }
 
 inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+// cudaFuncSetAttribute(kernel, MaxDynamicSharedMemorySize, bytes) once per kernel and device.
+template <typename Kernel>
+cudaError_t set_smem_once(Kernel kernel, int bytes, unsigned long long& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0ull;
+  if (__atomic_load_n(&done, __ATOMIC_RELAXED) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) __atomic_fetch_or(&done, bit, __ATOMIC_RELAXED);
+  return e;
+}
 
 // A launch whose set-up may overlap the end of the kernel before it on the stream.  Every kernel launched so
 // executes griddepcontrol.wait in every thread before its first global access, and so orders itself after
