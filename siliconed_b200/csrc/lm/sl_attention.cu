@@ -40,7 +40,6 @@ namespace sl {
 namespace {
 
 constexpr int kStep = 32;                 // tokens of a warp's step: two MMA tiles of 16
-constexpr int kLeastUnits = 2;            // of a share: a cut costs more than a step
 constexpr int kMaxBatch = 512;            // sequences of a launch
 
 struct Attention {
@@ -113,10 +112,22 @@ __device__ __forceinline__ void copy_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
 }
 
-// The share of work: CTA w of W takes units [w T / W, (w + 1) T / W); unit u belongs to CTA ((u + 1) W - 1) / T.
-__device__ __forceinline__ int64_t share_start(int64_t w, int64_t total, int64_t workers) { return w * total / workers; }
-__device__ __forceinline__ int64_t share_of(int64_t u, int64_t total, int64_t workers) {
-  return ((u + 1) * workers - 1) / total;
+// The shares of `total` units among `workers` CTAs: consecutive, the first `extra` of them one unit longer.  Counted in 32
+// bits (the launch sees to it): a 64-bit division takes as long as a step's products.
+struct Shares {
+  uint32_t workers, each, extra;
+  __device__ __forceinline__ uint32_t start(uint32_t w) const { return w * each + min(w, extra); }
+  __device__ __forceinline__ uint32_t of(uint32_t u) const {
+    const uint32_t longer = extra * (each + 1);
+    return u < longer ? u / (each + 1) : extra + (u - longer) / each;
+  }
+};
+
+// Adds one and returns the count before: what this CTA wrote before is seen by whoever counts after it.
+__device__ __forceinline__ uint32_t count_arrival(uint32_t* counter) {
+  uint32_t before;
+  asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+  return before;
 }
 
 // Geometry of a step's 32 tokens in shared memory: rows in order.  Lane (g, c) reads bytes 64 j + 16 c .. of the key rows
@@ -165,8 +176,9 @@ __global__ void __launch_bounds__(Shape<kDim, kE4m3, kNH, kWide>::kThreads, Shap
   constexpr int kPairs = kDim / 16;  // M tiles of O^T
 
   extern __shared__ __align__(128) uint8_t ring[];
-  __shared__ int64_t first_unit[kMaxBatch + 1];
-  __shared__ int64_t scan[kWarps];
+  __shared__ uint32_t first_unit[kMaxBatch + 1];
+  __shared__ int length[kMaxBatch];
+  __shared__ uint32_t scan[kWarps];
   __shared__ float part_m[kWarps][kRows], part_l[kWarps][kRows];
   __shared__ uint64_t arrived[kWarps][kSlots];
   __shared__ int last_flag, abort_flag;
@@ -182,36 +194,37 @@ __global__ void __launch_bounds__(Shape<kDim, kE4m3, kNH, kWide>::kThreads, Shap
   sc::pdl_wait();
 
   // Units of every sequence, summed: each thread takes a run of sequences.
-  const int hh = a.kv_heads * a.subs;
-  const int64_t room = static_cast<int64_t>(a.table_width) * a.page_size;
+  const uint32_t hh = a.kv_heads * a.subs;
+  const int room = a.table_width * a.page_size;
   {
     const int per = (a.batch + kThreads - 1) / kThreads;
     const int b0 = tid * per, b1 = min(a.batch, b0 + per);
-    int64_t mine = 0;
+    uint32_t own = 0;
     for (int b = b0; b < b1; ++b) {
-      int64_t len = a.lengths[b];
+      int len = a.lengths[b];
       if (len < 0 || len > room) {
         sc::record_error(a.err, kErrRange, kSiteAttentionLength);
         len = len < 0 ? 0 : room;
       }
-      first_unit[b] = mine;
-      mine += (len + kUnit - 1) / kUnit * hh;
+      length[b] = len;
+      first_unit[b] = own;
+      own += static_cast<uint32_t>(len + kUnit - 1) / kUnit * hh;
     }
-    int64_t sum = mine;
+    uint32_t sum = own;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
-      const int64_t v = __shfl_up_sync(0xFFFFFFFFu, sum, off);
+      const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, sum, off);
       if (lane >= off) sum += v;
     }
     if (lane == 31) scan[warp] = sum;
     __syncthreads();
-    int64_t before = sum - mine;
+    uint32_t before = sum - own;
     for (int w = 0; w < warp; ++w) before += scan[w];
     for (int b = b0; b < b1; ++b) first_unit[b] += before;
-    if (tid == kThreads - 1) first_unit[a.batch] = before + mine;
+    if (tid == kThreads - 1) first_unit[a.batch] = before + own;
     __syncthreads();
   }
-  const int64_t total = first_unit[a.batch];
+  const uint32_t total = first_unit[a.batch];
 
   // Sequences without tokens.
   for (int b = blockIdx.x; b < a.batch; b += gridDim.x)
@@ -222,11 +235,14 @@ __global__ void __launch_bounds__(Shape<kDim, kE4m3, kNH, kWide>::kThreads, Shap
         for (int i = tid; i < a.heads; i += kThreads) a.lse[static_cast<int64_t>(b) * a.heads + i] = -INFINITY;
     }
 
-  const int64_t workers = max(min(static_cast<int64_t>(gridDim.x), total / kLeastUnits), min(total, int64_t(1)));
-  if (blockIdx.x >= workers) return;
-  const int64_t u_begin = share_start(blockIdx.x, total, workers), u_end = share_start(blockIdx.x + 1, total, workers);
+  Shares shares;
+  shares.workers = min(gridDim.x, total);
+  if (blockIdx.x >= shares.workers) return;
+  shares.each = total / shares.workers;
+  shares.extra = total % shares.workers;
+  const uint32_t u_begin = shares.start(blockIdx.x), u_end = shares.start(blockIdx.x + 1);
 
-  for (int64_t u = u_begin; u < u_end;) {
+  for (uint32_t u = u_begin; u < u_end;) {
     // The sequence, key-value head and tile of query heads of unit u: the last sequence that starts at or before it
     // (sequences without tokens share their start with the next one).
     int lo = 0, hi = a.batch;
@@ -235,16 +251,15 @@ __global__ void __launch_bounds__(Shape<kDim, kE4m3, kNH, kWide>::kThreads, Shap
       if (first_unit[mid] <= u) lo = mid; else hi = mid;
     }
     const int b = lo;
-    const int64_t units = (first_unit[b + 1] - first_unit[b]) / hh;
-    const int64_t which = (u - first_unit[b]) / units;
-    const int64_t s0 = first_unit[b] + which * units, s1 = s0 + units;
+    const uint32_t units = (first_unit[b + 1] - first_unit[b]) / hh;
+    const uint32_t which = (u - first_unit[b]) / units;
+    const uint32_t s0 = first_unit[b] + which * units, s1 = s0 + units;
     const int kvh = static_cast<int>(which) / a.subs, sub = static_cast<int>(which) % a.subs;
     const int head0 = kvh * a.group + sub * kRows;             // first query head of the tile
     const int rows = min(kRows, a.group - sub * kRows);        // query heads of the tile
-    const int64_t stop = min(u_end, s1);
-    const int len = static_cast<int>(min(max(static_cast<int64_t>(a.lengths[b]), int64_t(0)), room));
-    const int t_begin = static_cast<int>((u - s0) * kUnit);
-    const int t_end = static_cast<int>(min(static_cast<int64_t>(len), (stop - s0) * kUnit));
+    const uint32_t stop = min(u_end, s1);
+    const int t_begin = static_cast<int>(u - s0) * kUnit;
+    const int t_end = min(length[b], static_cast<int>(stop - s0) * kUnit);
     const int32_t* table = a.table + static_cast<int64_t>(b) * a.table_width;
 
     // q as the B operand of S^T: query head g of each tile of 8, the dims in the order of the key loads.
@@ -624,21 +639,18 @@ __global__ void __launch_bounds__(Shape<kDim, kE4m3, kNH, kWide>::kThreads, Shap
     }
     if (!whole) {
       // The last of the context's CTAs adds the parts, in the order of the shares.
-      const int64_t wa = share_of(s0, total, workers), wb = share_of(s1 - 1, total, workers);
+      const uint32_t wa = shares.of(s0), wb = shares.of(s1 - 1);
       __syncthreads();
       if (tid == 0) {
-        __threadfence();  // after the barrier: the whole CTA's part
-        const uint32_t before = atomicAdd(a.counters + wa, 1u);
-        last_flag = before == static_cast<uint32_t>(wb - wa);
+        last_flag = count_arrival(a.counters + wa) == wb - wa;  // after the barrier: the whole CTA's part
         if (last_flag) a.counters[wa] = 0u;
-        __threadfence();
       }
       __syncthreads();
       if (last_flag) {
         // Part w lies in slot 0, but for the first one when that CTA began an earlier context.
         const int count = static_cast<int>(wb - wa) + 1;
-        const float* first = a.parts + (wa * 2 + (share_start(wa, total, workers) < s0 ? 1 : 0)) * kPartFloats;
-        const float* others = a.parts + wa * 2 * kPartFloats;
+        const float* first = a.parts + (static_cast<int64_t>(wa) * 2 + (shares.start(wa) < s0 ? 1 : 0)) * kPartFloats;
+        const float* others = a.parts + static_cast<int64_t>(wa) * 2 * kPartFloats;
         auto part_of = [&](int w) { return w == 0 ? first : others + static_cast<int64_t>(w) * 2 * kPartFloats; };
         const int d0 = (tid % kRun) * 4;
         // The first parts' sums are on their way while every part's factor exp(m_w - m) is formed.
@@ -777,6 +789,10 @@ extern "C" int sl_paged_attention(const uint16_t* q, const void* k_cache, const 
   if (pages > 0x7FFFFFFF || static_cast<double>(pages) * kv_heads * page_size >= 4294967295.0 ||
       static_cast<int64_t>(table_width) * page_size > 0x7FFF0000)
     return SL_INVALID_ARG;
+  // So are a launch's units of 128 tokens or more.
+  const int64_t most = 0x7FFFFFFFll / ((static_cast<int64_t>(table_width) * page_size + 127) / 128 * heads);
+  if (most < 1) return SL_INVALID_ARG;
+  const int per_launch = static_cast<int>(most < kMaxBatch ? most : kMaxBatch);
   if (batch == 0) return SL_OK;
   for (const void* p : {static_cast<const void*>(q), k_cache, v_cache, static_cast<const void*>(out),
                         static_cast<const void*>(workspace)})
@@ -797,7 +813,7 @@ extern "C" int sl_paged_attention(const uint16_t* q, const void* k_cache, const 
   if ((page_size & (page_size - 1)) == 0)
     for (shift = 0; (1 << shift) < page_size;) ++shift;
   const float scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
-  for (int b0 = 0; b0 < batch; b0 += kMaxBatch) {
+  for (int b0 = 0; b0 < batch; b0 += per_launch) {
     const int64_t at = static_cast<int64_t>(b0) * heads;
     const Attention a{q + at * head_dim,
                       k_cache,
@@ -806,7 +822,7 @@ extern "C" int sl_paged_attention(const uint16_t* q, const void* k_cache, const 
                       v_scale,
                       table + static_cast<int64_t>(b0) * table_width,
                       lengths + b0,
-                      batch - b0 < kMaxBatch ? batch - b0 : kMaxBatch,
+                      batch - b0 < per_launch ? batch - b0 : per_launch,
                       heads,
                       kv_heads,
                       group,
