@@ -369,11 +369,11 @@ __global__ void __launch_bounds__(Shape<kDim, kE4m3, kNH, kWide>::kThreads, Shap
     };
     // The oldest copy not yet used; null when it did not arrive in time.
     auto arrival = [&]() -> const uint8_t* {
-      const bool ok = sc::mbar_wait(&arrived[warp][take], (phases >> take) & 1, &abort_flag, a.err, kSiteAttentionCopy);
+      const bool ok = wait_warp(&arrived[warp][take], (phases >> take) & 1, &abort_flag, a.err, kSiteAttentionCopy);
       const uint8_t* at = mine + take * S::kSlotBytes;
       phases ^= 1u << take;
       take = take + 1 == kSlots ? 0 : take + 1;
-      return __all_sync(0xFFFFFFFFu, ok) ? at : nullptr;
+      return ok ? at : nullptr;
     };
 
     // Copy n is the keys of step n / 2 (n even) or its values (n odd); copy n + kSlots goes out when copy n has been used.

@@ -74,6 +74,31 @@ cudaError_t launch(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
 }
 
+// Waits for the phase of `bar` with parity `parity`, as sc::mbar_wait, but without reading the global timer until many
+// tries have failed: most waits here are short ones on a kernel's critical path.  Gives up (and raises `abort`) after
+// sc::kWaitLimitNs.
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* err, int site) {
+  unsigned long long since = 0;
+  for (uint32_t i = 1;; ++i) {
+    if (sc::mbar_try_wait(bar, parity)) return true;
+    if ((i & 255u) != 0) continue;
+    if (*abort) return false;
+    const unsigned long long now = sc::global_ns();
+    if (since == 0) since = now;
+    if (now - since > sc::kWaitLimitNs) {
+      sc::record_error(err, sc::kErrTimeout, site);
+      *abort = 1;
+      return false;
+    }
+  }
+}
+
+// A warp's wait: all or none.
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort, int* err, int site) {
+  const bool got = wait(bar, parity, abort, err, site);
+  return __all_sync(0xFFFFFFFFu, got) != 0;
+}
+
 __device__ __forceinline__ float from_bf16(uint32_t u) { return __uint_as_float(u << 16); }
 
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {

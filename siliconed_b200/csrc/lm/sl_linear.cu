@@ -4,70 +4,406 @@
 //
 // The scales change every 128 values of K, so an accumulator cannot run over all of K: the tensor cores produce one
 // block's partial product in TMEM (tcgen05.mma kind::f8f6f4, four MMAs of K 32), and the epilogue warps multiply it
-// by its scales and add it to fp32 sums in registers while the MMAs of the next blocks run into other TMEM buffers.
+// by its scales and add it to fp32 sums in registers while the MMAs of the next block run into the other TMEM buffer.
 //
-// One CTA per 128 x 128 tile of y.  Warp 0: TMA (a and w tiles of 128 rows x 128 bytes, 128-byte swizzle, a ring of
-// kStages); warp 1: TMEM and MMA issue; warps 2-5: one row of the tile a thread.  Rows past m or n and values past k
-// arrive as zeros.  Every wait is bounded; no load uses cluster multicast.
+// Two kernels, by the count of rows (choose()):
+//
+// - linear_pair: a cluster of two CTAs owns tiles of 256 x 256 of y (tcgen05.mma.cta_group::2), persistent over the
+//   tiles.  Each CTA loads its own 128 rows of a and of w by TMA (128-byte swizzle).  The tile leaves through shared
+//   memory by TMA stores, which run under the next tile's blocks.  What bounds it is a block's round trip through its TMEM
+//   buffer: 4 MMAs (650 cycles beside the epilogue's work), their commit (350), the partial read by 16 warps (450) and the
+//   buffer's release to the MMA thread (400), some 1900 cycles for the two buffers that 256 columns leave.  [4096, 3840] x
+//   [3840, 10240]: 186 us, 1730 TFLOP/s; without the epilogue's arithmetic 134 us, the loads take less.  (Tiles of 256 x
+//   128 with four buffers: 198 us, their MMAs read shared memory half again as often.  fma.rn.f32x2 for the sums: 293 us,
+//   pairs of registers moved together.  One issuing thread: 212 us.)
+// - linear_swap: for few rows, bound by reading the weight.  The operands change places: 128 weight rows are the MMA's
+//   M and the rows of a, in tiles of up to 128, its N, so that no MMA row or TMEM column is padding; K is cut over the
+//   CTAs of a cluster, whose partials meet through distributed shared memory and are added in rank order.
+//
+// Rows past m or n and values past k arrive as zeros.  Every wait is bounded; no load uses cluster multicast.
 #include "sl_common.cuh"
 
 namespace sl {
 namespace {
 
-constexpr int BM = 128, BN = 128, BK = 128;
-constexpr int kStages = 5;
-constexpr int kBuffers = 4;                // TMEM buffers of BN columns
-constexpr int kTileBytes = BM * BK;
-constexpr int kThreads = 192;
-constexpr uint32_t kTmemCols = kBuffers * BN;
-
-struct __align__(1024) Smem {
-  uint8_t a[kStages][kTileBytes];
-  uint8_t w[kStages][kTileBytes];
-  uint64_t full[kStages], empty[kStages];
-  uint64_t part_full[kBuffers], part_empty[kBuffers];
-  uint64_t drain;
-  uint32_t tmem_base;
-  int abort;
-};
-
-constexpr size_t kSmemBytes = sizeof(Smem) + 1024;
-static_assert(kSmemBytes <= 227 * 1024, "shared memory per CTA");
+constexpr int BK = 128;         // values of K under one scale: a stage, 128 bytes a row
+constexpr int kRowBytes = BK;
 
 // kind::f8f6f4 with e4m3 operands, both K-major, fp32 accumulation.
 __host__ __device__ constexpr uint32_t idesc_e4m3(int m, int n) {
   return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
+template <bool kPair>
 __device__ __forceinline__ void mma_e4m3(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                          uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-      : "memory");
+  if (kPair)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
 }
 
-template <bool kF32Out>
+// Waits for this thread's TMEM loads; the values it loaded cannot be used above it.
+__device__ __forceinline__ void tmem_wait_32(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
+}
+
+__device__ __forceinline__ uint64_t pair_of(uint32_t lo, uint32_t hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
+  return v;
+}
+__device__ __forceinline__ float2 floats_of(uint64_t v) {
+  uint32_t lo, hi;
+  asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(v));
+  return make_float2(__uint_as_float(lo), __uint_as_float(hi));
+}
+// Two fp32 a * b + c, each rounded once.
+__device__ __forceinline__ void fma2(uint64_t& c, uint64_t a, uint64_t b) {
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(a), "l"(b));
+}
+
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(src), "r"(c0), "r"(c1)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+template <int kLeft>
+__device__ __forceinline__ void bulk_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kLeft) : "memory");
+}
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+__device__ __forceinline__ float bias_at(const uint16_t* bias, int col, int n) {
+  return bias != nullptr && col < n ? from_bf16(bias[col]) : 0.0f;
+}
+
+// ------------------------------------------------------------------------------------------ many rows
+
+namespace pair {
+
+constexpr int BM = 128;                   // rows of a per CTA, 256 a pair
+constexpr int BN = 256, BNH = BN / 2;     // columns of a pair tile; rows of w each CTA loads
+constexpr int kStages = 5;
+constexpr int kTileBytes = BM * kRowBytes;
+constexpr int kEpiWarp0 = 4, kEpiWarps = 8;
+constexpr int kThreads = (kEpiWarp0 + kEpiWarps) * 32;
+// Registers a thread after the split: the sums (128), three loads (96) and addresses; the TMA and MMA warps'
+// group gives up what it does not need.  The launch checks that the kernel was built with at least their sum.
+constexpr int kEpiRegisters = 232, kOtherRegisters = 40;
+constexpr int kLaunchRegisters = (kOtherRegisters + 2 * kEpiRegisters + 2) / 3;
+constexpr uint32_t kTmemCols = 512;       // two partial products of 256 columns
+constexpr int kBoxBytes = 32 * 128;       // 32 rows of 128 bytes of y: a TMA store
+
+struct __align__(1024) Smem {
+  uint8_t a[kStages][kTileBytes];
+  uint8_t w[kStages][kTileBytes];
+  uint8_t out[kEpiWarps][2][kBoxBytes];
+  uint64_t full[kStages];                  // the leader's: both CTAs' bytes of the stage landed
+  uint64_t done[kStages];                  // the stage's MMAs completed: its partial is there, the stage is free
+  uint64_t part_empty[2];                  // the leader's: both CTAs' epilogues have read the buffer
+  uint64_t drain[2];
+  uint32_t tmem_base;
+  int abort;
+};
+constexpr size_t kSmemBytes = sizeof(Smem) + 1024;
+static_assert(kSmemBytes <= 227 * 1024, "shared memory per CTA");
+
+// kTmaOut: y's rows start on 16 bytes, so that whole boxes leave by TMA.
+template <bool kF32Out, bool kTmaOut>
 __global__ void __launch_bounds__(kThreads, 1)
-    linear_block_fp8_k(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_w,
-                       const float* __restrict__ a_scales, const float* __restrict__ w_scales,
-                       const uint16_t* __restrict__ bias, void* __restrict__ y, int m, int n, int k_blocks, int* err) {
+    linear_pair(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_w,
+                const __grid_constant__ CUtensorMap tm_y, const float* __restrict__ a_scales,
+                const float* __restrict__ w_scales, const uint16_t* __restrict__ bias, void* __restrict__ y, int m, int n,
+                int k_blocks, int m_tiles, int n_tiles, int* err) {
   extern __shared__ uint8_t smem_raw[];
   Smem& s = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int m0 = blockIdx.y * BM, n0 = blockIdx.x * BN;
+  const uint32_t rank = sc::cluster_ctarank();
+  const bool leader = rank == 0;
+  const int first = blockIdx.x >> 1, pairs = gridDim.x >> 1, tiles = m_tiles * n_tiles;
   volatile int* abort = &s.abort;
   sc::pdl_launch_dependents();
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
       sc::mbar_init(&s.full[i], 1);
+      sc::mbar_init(&s.done[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      sc::mbar_init(&s.part_empty[i], 2 * kEpiWarps);
+      sc::mbar_init(&s.drain[i], 1);
+    }
+    s.abort = 0;
+    sc::fence_mbar_init();
+    sc::prefetch_tensormap(&tm_a);
+    sc::prefetch_tensormap(&tm_w);
+    if (kTmaOut) sc::prefetch_tensormap(&tm_y);
+  }
+  if (warp == 1) {
+    sc::tmem_alloc_pair(&s.tmem_base, kTmemCols);
+    sc::tmem_relinquish_pair();
+  }
+  __syncwarp();
+  sc::tc_fence_before();
+  sc::cluster_barrier();
+  sc::tc_fence_after();
+  const uint32_t tmem = s.tmem_base;
+  sc::pdl_wait();
+
+  if (warp >= kEpiWarp0) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpiRegisters));
+    // One row of the tile a thread, 128 of its columns: one scale block of w.
+    const int ew = warp - kEpiWarp0, quarter = warp & 3, half = ew >> 2;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * BNH;
+    int buf = 0, stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int tile = first; tile < tiles && ok; tile += pairs) {
+      int mt, nt;
+      sc::tile_coords(tile, m_tiles, n_tiles, mt, nt);
+      const int row0 = (mt * 2 + static_cast<int>(rank)) * BM + quarter * 32, row = row0 + lane;
+      const int col0 = nt * BN + half * BNH;
+      // The last tile's second half may have no columns: any block's scales do.
+      const float* sa = a_scales + static_cast<int64_t>(min(row, m - 1)) * k_blocks;
+      const float* sw = w_scales + static_cast<int64_t>(min(col0, n - 1) / BK) * k_blocks;
+      float acc[BNH];
+#pragma unroll
+      for (int j = 0; j < BNH; ++j) acc[j] = 0.0f;
+      // The scales are asked for two blocks ahead, into registers of their own for even and odd blocks: handed from one
+      // to the next they would have to arrive first (one block then took 2000 cycles instead of 750).
+      float a_even = sa[0], w_even = sw[0], a_odd = sa[min(1, k_blocks - 1)], w_odd = sw[min(1, k_blocks - 1)];
+      const auto add_block = [&](int kb, float& a_scale, float& w_scale) {
+        if (!(ok = wait_warp(&s.done[stage], phase, abort, err, kSiteLinearSum))) return;
+        sc::tc_fence_after();
+        const float f = a_scale * w_scale;
+        const int next = min(kb + 2, k_blocks - 1);
+        a_scale = sa[next];
+        w_scale = sw[next];
+        uint32_t r[3][32];
+        const auto load = [&](int q, uint32_t(&into)[32]) { sc::tmem_ld_32(lanes + buf * BN + q * 32, into); };
+        const auto add = [&](int q, const uint32_t(&part)[32]) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) acc[q * 32 + j] = fmaf(__uint_as_float(part[j]), f, acc[q * 32 + j]);
+        };
+        load(0, r[0]);
+        load(1, r[1]);
+        load(2, r[2]);
+        tmem_wait_32(r[0]);
+        tmem_wait_32(r[1]);
+        tmem_wait_32(r[2]);
+        add(0, r[0]);
+        load(3, r[0]);
+        tmem_wait_32(r[0]);
+        // All of the partial is in registers: its buffer is free.
+        sc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) sc::mbar_arrive_cluster(sc::peer_addr(&s.part_empty[buf], 0));
+        add(1, r[1]);
+        add(2, r[2]);
+        add(3, r[0]);
+        buf ^= 1;
+        if (++stage == kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      };
+      for (int kb = 0; kb < k_blocks && ok; kb += 2) {
+        add_block(kb, a_even, w_even);
+        if (kb + 1 < k_blocks && ok) add_block(kb + 1, a_odd, w_odd);
+      }
+      if (!ok) break;
+      if (kTmaOut) {
+        constexpr int kBoxCols = kF32Out ? 32 : 64;  // 128 bytes
+        uint8_t* out = &s.out[ew][0][0];
+#pragma unroll
+        for (int b = 0; b < BNH / kBoxCols; ++b) {
+          if (lane == 0) bulk_wait_read<1>();  // the store of two boxes ago has read this half
+          __syncwarp();
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            uint4 v;
+            if (kF32Out) {
+              const int j = b * 32 + q * 4;
+              v = make_uint4(__float_as_uint(acc[j] + bias_at(bias, col0 + j, n)), __float_as_uint(acc[j + 1] + bias_at(bias, col0 + j + 1, n)),
+                             __float_as_uint(acc[j + 2] + bias_at(bias, col0 + j + 2, n)), __float_as_uint(acc[j + 3] + bias_at(bias, col0 + j + 3, n)));
+            } else {
+              float x[8];
+#pragma unroll
+              for (int t = 0; t < 8; ++t) x[t] = acc[b * 64 + q * 8 + t] + bias_at(bias, col0 + b * 64 + q * 8 + t, n);
+              v = pack8(x);
+            }
+            *reinterpret_cast<uint4*>(out + (b & 1) * kBoxBytes + lane * 128 + ((q ^ (lane & 7)) << 4)) = v;
+          }
+          sc::fence_async_shared();
+          __syncwarp();
+          if (lane == 0) {
+            if (row0 < m && col0 + b * kBoxCols < n)
+              tma_store_2d(&tm_y, sc::smem_u32(out + (b & 1) * kBoxBytes), col0 + b * kBoxCols, row0);
+            bulk_commit();
+          }
+        }
+      } else if (row < m) {
+        const int64_t at = static_cast<int64_t>(row) * n + col0;
+#pragma unroll
+        for (int j = 0; j < BNH; ++j)
+          if (col0 + j < n) {
+            const float v = acc[j] + bias_at(bias, col0 + j, n);
+            if (kF32Out)
+              static_cast<float*>(y)[at + j] = v;
+            else
+              static_cast<__nv_bfloat16*>(y)[at + j] = __float2bfloat16_rn(v);
+          }
+      }
+    }
+    if (kTmaOut && lane == 0) bulk_wait_all();
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
+    if (warp == 0) {
+      // TMA: each CTA its own halves, both CTAs' bytes counted on the leader's barrier.
+      if (lane == 0) {
+        int stage = 0;
+        uint32_t phase = 0, issued = 0, last_parity = 0;
+        bool ok = true;
+        for (int tile = first; tile < tiles && ok; tile += pairs) {
+          int mt, nt;
+          sc::tile_coords(tile, m_tiles, n_tiles, mt, nt);
+          const int row0 = (mt * 2 + static_cast<int>(rank)) * BM, col0 = nt * BN + static_cast<int>(rank) * BNH;
+          for (int kb = 0; kb < k_blocks; ++kb) {
+            if (!wait(&s.done[stage], phase ^ 1u, abort, err, kSiteLinearLoad)) {
+              ok = false;
+              break;
+            }
+            if (leader) sc::mbar_arrive_expect_tx(&s.full[stage], 4 * kTileBytes);
+            const uint32_t bar = sc::peer_addr(&s.full[stage], 0);
+            sc::tma_load_2d_pair(s.a[stage], &tm_a, bar, kb * BK, row0);
+            sc::tma_load_2d_pair(s.w[stage], &tm_w, bar, kb * BK, col0);
+            issued |= 1u << stage;
+            last_parity = (last_parity & ~(1u << stage)) | (phase << stage);
+            if (++stage == kStages) {
+              stage = 0;
+              phase ^= 1u;
+            }
+          }
+        }
+        if (leader)
+          for (int st = 0; st < kStages; ++st)
+            if (issued & (1u << st)) sc::mbar_wait_drain(&s.full[st], (last_parity >> st) & 1u);
+      }
+    } else if (warp <= 2) {
+      // Two threads issue the MMAs, block by block in turns, each into its own TMEM buffer: one's commit and waits (some
+      // 400 cycles a block) run under the other's MMAs.
+      if (leader && lane == 0) {
+        constexpr uint32_t idesc = idesc_e4m3(2 * BM, BN);
+        const int buf = warp - 1;
+        const int blocks = (tiles - first + pairs - 1) / pairs * k_blocks;  // of this pair's tiles
+        int stage = buf;
+        uint32_t phase = 0, buf_phase = 0;
+        for (int g = buf; g < blocks; g += 2) {
+          if (!wait(&s.part_empty[buf], buf_phase ^ 1u, abort, err, kSiteLinearBuffer) ||
+              !wait(&s.full[stage], phase, abort, err, kSiteLinearMma))
+            break;
+          sc::tc_fence_after();
+          const uint32_t a0 = sc::smem_u32(s.a[stage]), b0 = sc::smem_u32(s.w[stage]);
+#pragma unroll
+          for (int kk = 0; kk < BK / 32; ++kk)
+            mma_e4m3<true>(tmem + static_cast<uint32_t>(buf * BN), sc::umma_desc_sw128(a0 + kk * 32),
+                           sc::umma_desc_sw128(b0 + kk * 32), idesc, kk != 0 ? 1u : 0u);
+          sc::tc_commit_pair_both(&s.done[stage], 0x3);
+          buf_phase ^= 1u;
+          stage += 2;
+          if (stage >= kStages) {
+            stage -= kStages;
+            phase ^= 1u;
+          }
+        }
+        sc::tc_commit_pair(sc::peer_addr(&s.drain[buf], 0));
+        sc::mbar_wait_drain(&s.drain[buf], 0);
+      }
+    }
+  }
+  // Neither CTA leaves while the pair's MMAs, TMEM or barriers may still reach its memory.
+  __syncwarp();
+  sc::tc_fence_before();
+  sc::cluster_barrier();
+  if (warp == 1) {
+    sc::tc_fence_after();
+    sc::tmem_dealloc_pair(tmem, kTmemCols);
+  }
+}
+
+}  // namespace pair
+
+// ------------------------------------------------------------------------------------------ few rows
+
+namespace swap {
+
+constexpr int BN = 128;                   // rows of w (columns of y) a CTA
+constexpr int kMostRows = 128;            // rows of a, the MMA's N
+constexpr int kWBytes = BN * kRowBytes;
+constexpr int kMostStages = 6;
+constexpr int kRingBytes = 104 * 1024;    // two CTAs an SM
+constexpr int kEpiWarp0 = 2, kEpiWarps = 4, kEpiThreads = kEpiWarps * 32;
+constexpr int kThreads = (kEpiWarp0 + kEpiWarps) * 32;
+
+struct Control {
+  uint64_t full[kMostStages], empty[kMostStages];
+  uint64_t part_full[2], part_empty[2];
+  uint64_t drain;
+  uint32_t tmem_base;
+  int abort;
+  float factors[2][kMostRows];            // sa * sw of the block, by its parity
+};
+constexpr size_t kSmemBytes = kRingBytes + 1024;
+static_assert(kMostRows * BN * 4 <= kRingBytes, "a partial fits the ring");
+
+// kRows: the sums' registers (16, 32, 64 or 128); `rows` <= kRows is the tile's count, a multiple of 16, and the rows of
+// a's TMA box.
+template <bool kF32Out, int kRows>
+__global__ void __launch_bounds__(kThreads, 2)
+    linear_swap(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_w,
+                const float* __restrict__ a_scales, const float* __restrict__ w_scales,
+                const uint16_t* __restrict__ bias, void* __restrict__ y, int m, int n, int k_blocks, int rows, int stages,
+                int* err) {
+  constexpr int kBuffers = 2;
+  constexpr uint32_t kTmemCols = kBuffers * kRows;
+  constexpr int kChunk = kRows < 32 ? 16 : 32;           // TMEM columns of a load
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ Control s;
+  uint8_t* const ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int stage_bytes = kWBytes + rows * kRowBytes;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = sc::cluster_ctarank();
+  uint32_t parts;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(parts));
+  const int tile = static_cast<int>(blockIdx.x / parts), n0 = tile * BN, m0 = blockIdx.y * rows;
+  const int kb0 = static_cast<int>(rank * static_cast<uint32_t>(k_blocks) / parts);
+  const int kb1 = static_cast<int>((rank + 1) * static_cast<uint32_t>(k_blocks) / parts);
+  volatile int* abort = &s.abort;
+  sc::pdl_launch_dependents();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < stages; ++i) {
+      sc::mbar_init(&s.full[i], 1);
       sc::mbar_init(&s.empty[i], 1);
     }
-    for (int i = 0; i < kBuffers; ++i) {
+    for (int i = 0; i < 2; ++i) {
       sc::mbar_init(&s.part_full[i], 1);
-      sc::mbar_init(&s.part_empty[i], 4);
+      sc::mbar_init(&s.part_empty[i], kEpiWarps);
     }
     sc::mbar_init(&s.drain, 1);
     s.abort = 0;
@@ -89,39 +425,39 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       int stage = 0;
       uint32_t phase = 0, issued = 0, last_parity = 0;
-      for (int kb = 0; kb < k_blocks; ++kb) {
-        if (!sc::mbar_wait(&s.empty[stage], phase ^ 1u, abort, err, kSiteLinearLoad)) break;
-        sc::mbar_arrive_expect_tx(&s.full[stage], 2 * kTileBytes);
-        sc::tma_load_2d(s.a[stage], &tm_a, &s.full[stage], kb * BK, m0);
-        sc::tma_load_2d(s.w[stage], &tm_w, &s.full[stage], kb * BK, n0);
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!wait(&s.empty[stage], phase ^ 1u, abort, err, kSiteLinearLoad)) break;
+        sc::mbar_arrive_expect_tx(&s.full[stage], stage_bytes);
+        sc::tma_load_2d(ring + stage * stage_bytes, &tm_w, &s.full[stage], kb * BK, n0);
+        sc::tma_load_2d(ring + stage * stage_bytes + kWBytes, &tm_a, &s.full[stage], kb * BK, m0);
         issued |= 1u << stage;
         last_parity = (last_parity & ~(1u << stage)) | (phase << stage);
-        if (++stage == kStages) {
+        if (++stage == stages) {
           stage = 0;
           phase ^= 1u;
         }
       }
-      for (int st = 0; st < kStages; ++st)
+      for (int st = 0; st < stages; ++st)
         if (issued & (1u << st)) sc::mbar_wait_drain(&s.full[st], (last_parity >> st) & 1u);
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      constexpr uint32_t idesc = idesc_e4m3(BM, BN);
+      const uint32_t idesc = idesc_e4m3(BN, rows);
       int stage = 0, buf = 0;
       uint32_t phase = 0, buf_phase = 0;
-      for (int kb = 0; kb < k_blocks; ++kb) {
-        if (!sc::mbar_wait(&s.part_empty[buf], buf_phase ^ 1u, abort, err, kSiteLinearBuffer) ||
-            !sc::mbar_wait(&s.full[stage], phase, abort, err, kSiteLinearMma))
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!wait(&s.part_empty[buf], buf_phase ^ 1u, abort, err, kSiteLinearBuffer) ||
+            !wait(&s.full[stage], phase, abort, err, kSiteLinearMma))
           break;
         sc::tc_fence_after();
-        const uint32_t a0 = sc::smem_u32(s.a[stage]), b0 = sc::smem_u32(s.w[stage]);
+        const uint32_t w0 = sc::smem_u32(ring + stage * stage_bytes), a0 = w0 + kWBytes;
 #pragma unroll
         for (int kk = 0; kk < BK / 32; ++kk)
-          mma_e4m3(tmem + static_cast<uint32_t>(buf * BN), sc::umma_desc_sw128(a0 + kk * 32), sc::umma_desc_sw128(b0 + kk * 32),
-                   idesc, kk != 0 ? 1u : 0u);
+          mma_e4m3<false>(tmem + static_cast<uint32_t>(buf * kRows), sc::umma_desc_sw128(w0 + kk * 32),
+                          sc::umma_desc_sw128(a0 + kk * 32), idesc, kk != 0 ? 1u : 0u);
         sc::tc_commit(&s.empty[stage]);
         sc::tc_commit(&s.part_full[buf]);
-        if (++stage == kStages) {
+        if (++stage == stages) {
           stage = 0;
           phase ^= 1u;
         }
@@ -134,30 +470,56 @@ __global__ void __launch_bounds__(kThreads, 1)
       sc::mbar_wait_drain(&s.drain, 0);
     }
   } else {
-    const int ew = warp & 3;  // a warp reads the TMEM lanes of its rank modulo 4
-    const int row = m0 + ew * 32 + lane;
-    const float* sa = a_scales + static_cast<int64_t>(min(row, m - 1)) * k_blocks;
-    const float* sw = w_scales + static_cast<int64_t>(blockIdx.x) * k_blocks;
-    float acc[BN];
+    // One column of y a thread; the block's factors sa * sw come through shared memory, a block ahead of their use.
+    const int et = threadIdx.x - kEpiWarp0 * 32, quarter = warp & 3;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    const float* sw = w_scales + static_cast<int64_t>(tile) * k_blocks;
+    const bool owns = et < rows && m0 + et < m;
+    const float* sa = a_scales + static_cast<int64_t>(owns ? m0 + et : 0) * k_blocks;
+    uint64_t acc[kRows / 2];
 #pragma unroll
-    for (int j = 0; j < BN; ++j) acc[j] = 0.0f;
+    for (int j = 0; j < kRows / 2; ++j) acc[j] = 0;
+    // Sums of the partial of every block; a wait that gave up leaves the sums as they are, but the loop goes on, so
+    // that every warp meets the others at each block's barrier.
+    // The scales are asked for two blocks ahead, into registers of their own for even and odd blocks.
+    const auto scale_at = [&](const float* p, int kb) { return owns && kb < kb1 ? p[kb] : 0.0f; };
+    float a_even = scale_at(sa, kb0), w_even = scale_at(sw, kb0), a_odd = scale_at(sa, kb0 + 1), w_odd = scale_at(sw, kb0 + 1);
     int buf = 0;
     uint32_t phase = 0;
-    bool ok = true;
-    for (int kb = 0; kb < k_blocks; ++kb) {
-      const float f = sa[kb] * sw[kb];
-      int got = 0;
-      if (lane == 0) got = sc::mbar_wait(&s.part_full[buf], phase, abort, err, kSiteLinearSum) ? 1 : 0;
-      ok = __shfl_sync(0xFFFFFFFFu, got, 0) != 0;
-      if (!ok) break;
+    const auto add_block = [&](int kb, float& a_scale, float& w_scale) {
+      if (et < kRows) s.factors[kb & 1][et] = a_scale * w_scale;
+      a_scale = scale_at(sa, kb + 2);
+      w_scale = scale_at(sw, kb + 2);
+      sc::named_barrier_sync(1, kEpiThreads);
+      const float* f = s.factors[kb & 1];
+      const bool ok = wait_warp(&s.part_full[buf], phase, abort, err, kSiteLinearSum);
       sc::tc_fence_after();
+      if (ok) {
 #pragma unroll
-      for (int q = 0; q < BN / 32; ++q) {
-        uint32_t r[32];
-        sc::tmem_ld_32(tmem + (static_cast<uint32_t>(ew * 32) << 16) + buf * BN + q * 32, r);
-        sc::tmem_wait_ld();
+        for (int q = 0; q < kRows / kChunk; ++q) {
+          if (q * kChunk >= rows) break;
+          uint32_t r[32];
+          if (kChunk == 32) {
+            sc::tmem_ld_32(lanes + buf * kRows + q * 32, r);
+          } else {
+            asm volatile(
+                "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+                "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                  "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                : "r"(lanes + buf * kRows + q * 16)
+                : "memory");
 #pragma unroll
-        for (int j = 0; j < 32; ++j) acc[q * 32 + j] += f * __uint_as_float(r[j]);
+            for (int j = 16; j < 32; ++j) r[j] = 0;
+          }
+          tmem_wait_32(r);
+#pragma unroll
+          for (int j = 0; j < kChunk; j += 4) {
+            const float4 fv = *reinterpret_cast<const float4*>(f + q * kChunk + j);
+            fma2(acc[(q * kChunk + j) / 2], pair_of(r[j], r[j + 1]), pair_of(__float_as_uint(fv.x), __float_as_uint(fv.y)));
+            fma2(acc[(q * kChunk + j) / 2 + 1], pair_of(r[j + 2], r[j + 3]), pair_of(__float_as_uint(fv.z), __float_as_uint(fv.w)));
+          }
+        }
       }
       sc::tc_fence_before();
       __syncwarp();
@@ -166,47 +528,92 @@ __global__ void __launch_bounds__(kThreads, 1)
         buf = 0;
         phase ^= 1u;
       }
+    };
+    for (int kb = kb0; kb < kb1; kb += 2) {
+      add_block(kb, a_even, w_even);
+      if (kb + 1 < kb1) add_block(kb + 1, a_odd, w_odd);
     }
-    if (ok && row < m) {
-      const int64_t at = static_cast<int64_t>(row) * n + n0;
-      const bool wide = n % 8 == 0;  // rows of y start on 16 bytes
+    const int col = quarter * 32 + lane;
+    if (parts == 1) {
+      const float add = bias_at(bias, n0 + col, n);
+      if (n0 + col < n) {
 #pragma unroll
-      for (int j = 0; j < BN; j += 8) {
-        float v[8];
-#pragma unroll
-        for (int t = 0; t < 8; ++t) {
-          v[t] = acc[j + t];
-          if (bias != nullptr && n0 + j + t < n) v[t] += from_bf16(bias[n0 + j + t]);
-        }
-        if (wide && n0 + j < n) {
-          if (kF32Out) {
-            float4* o = reinterpret_cast<float4*>(static_cast<float*>(y) + at + j);
-            o[0] = make_float4(v[0], v[1], v[2], v[3]);
-            o[1] = make_float4(v[4], v[5], v[6], v[7]);
-          } else {
-            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(y) + at + j) = pack8(v);
+        for (int j = 0; j < kRows; ++j)
+          if (j < rows && m0 + j < m) {
+            const float2 p = floats_of(acc[j / 2]);
+            const float v = (j & 1 ? p.y : p.x) + add;
+            const int64_t at = static_cast<int64_t>(m0 + j) * n + n0 + col;
+            if (kF32Out)
+              static_cast<float*>(y)[at] = v;
+            else
+              static_cast<__nv_bfloat16*>(y)[at] = __float2bfloat16_rn(v);
           }
-        } else if (!wide) {
-#pragma unroll
-          for (int t = 0; t < 8; ++t)
-            if (n0 + j + t < n) {
-              if (kF32Out)
-                static_cast<float*>(y)[at + j + t] = v[t];
-              else
-                static_cast<__nv_bfloat16*>(y)[at + j + t] = __float2bfloat16_rn(v[t]);
-            }
-        }
       }
+    } else {
+      // Over the ring: every copy has arrived and every MMA has read it, or the wait for the last partial gave up and
+      // the kernel's error says so.
+      float* part = reinterpret_cast<float*>(ring);
+#pragma unroll
+      for (int j = 0; j < kRows; ++j)
+        if (j < rows) {
+          const float2 p = floats_of(acc[j / 2]);
+          part[j * BN + col] = j & 1 ? p.y : p.x;
+        }
     }
   }
   __syncwarp();
   sc::tc_fence_before();
-  __syncthreads();
+  if (parts > 1) {
+    // Every CTA adds a share of the rows, in rank order: the same sums whichever CTA adds them.
+    sc::cluster_barrier();
+    const int cp = threadIdx.x % (BN / 2), group = threadIdx.x / (BN / 2);
+    const int lo = static_cast<int>(rank) * rows / static_cast<int>(parts), hi = static_cast<int>(rank + 1) * rows / static_cast<int>(parts);
+    const int col = n0 + 2 * cp;
+    const float b0 = bias_at(bias, col, n), b1 = bias_at(bias, col + 1, n);
+    const bool both = n % 2 == 0 && col + 1 < n;
+    for (int t = lo + group; t < hi && m0 + t < m; t += kThreads / (BN / 2)) {
+      const float* mine = reinterpret_cast<const float*>(ring) + t * BN + 2 * cp;
+      float2 sum = make_float2(0.0f, 0.0f);
+      for (uint32_t q = 0; q < parts; ++q) {
+        float2 v;
+        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(sc::peer_addr(mine, q)) : "memory");
+        sum.x += v.x;
+        sum.y += v.y;
+      }
+      sum.x += b0;
+      sum.y += b1;
+      const int64_t at = static_cast<int64_t>(m0 + t) * n + col;
+      if (kF32Out) {
+        float* o = static_cast<float*>(y) + at;
+        if (both) {
+          *reinterpret_cast<float2*>(o) = sum;
+        } else {
+          if (col < n) o[0] = sum.x;
+          if (col + 1 < n) o[1] = sum.y;
+        }
+      } else {
+        __nv_bfloat16* o = static_cast<__nv_bfloat16*>(y) + at;
+        if (both) {
+          *reinterpret_cast<uint32_t*>(o) = pack_bf16x2(sum.x, sum.y);
+        } else {
+          if (col < n) o[0] = __float2bfloat16_rn(sum.x);
+          if (col + 1 < n) o[1] = __float2bfloat16_rn(sum.y);
+        }
+      }
+    }
+    sc::cluster_barrier();  // the partials stay until the other CTAs have read them
+  } else {
+    __syncthreads();
+  }
   if (warp == 1) {
     sc::tc_fence_after();
     sc::tmem_dealloc(tmem, kTmemCols);
   }
 }
+
+}  // namespace swap
+
+// ------------------------------------------------------------------------------------------ the launch
 
 typedef CUresult (*encode_fn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -224,15 +631,127 @@ encode_fn encoder() {
   return fn;
 }
 
-// [rows][k] bytes with boxes of 128 values x `box` rows, 128-byte swizzle, zeros outside.
-bool make_map(CUtensorMap* map, encode_fn enc, const uint8_t* base, int64_t rows, int64_t k, int box) {
-  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows)};
-  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(k)};
-  const cuuint32_t boxes[2] = {static_cast<cuuint32_t>(BK), static_cast<cuuint32_t>(box)};
+// A row-major [rows][cols] matrix in boxes of 128 bytes x `box` rows, 128-byte swizzle, zeros outside.
+bool make_map(CUtensorMap* map, encode_fn enc, CUtensorMapDataType type, int size, const void* base, int64_t rows, int64_t cols,
+              int box) {
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols) * size};
+  const cuuint32_t boxes[2] = {static_cast<cuuint32_t>(128 / size), static_cast<cuuint32_t>(box)};
   const cuuint32_t estr[2] = {1, 1};
-  return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(base), dims, strides, boxes, estr,
-             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return enc(map, type, 2, const_cast<void*>(base), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return n;
+}
+
+struct Product {
+  const uint8_t *a, *w;
+  const float *a_scales, *w_scales;
+  const uint16_t* bias;
+  int64_t m, n, k;
+  void* y;
+  bool f32;
+  int k_blocks, sms;
+  encode_fn enc;
+  int* err;
+  cudaStream_t stream;
+};
+
+template <typename... Params, typename... Args>
+cudaError_t launch_cluster(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t stream,
+                           Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+
+template <bool kF32Out, bool kTmaOut>
+cudaError_t launch_pair_as(const Product& p) {
+  using namespace pair;
+  auto kernel = linear_pair<kF32Out, kTmaOut>;
+  static unsigned long long configured = 0;
+  if (const cudaError_t e = set_smem_once(kernel, static_cast<int>(kSmemBytes), configured); e != cudaSuccess) return e;
+  static const int registers = [kernel] {
+    cudaFuncAttributes attr;
+    return cudaFuncGetAttributes(&attr, kernel) == cudaSuccess ? attr.numRegs : 0;
+  }();
+  if (registers < kLaunchRegisters) return cudaErrorLaunchOutOfResources;
+  CUtensorMap ta, tw, ty = {};
+  if (!make_map(&ta, p.enc, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.a, p.m, p.k, BM) ||
+      !make_map(&tw, p.enc, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.w, p.n, p.k, BNH) ||
+      (kTmaOut && !make_map(&ty, p.enc, kF32Out ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                            kF32Out ? 4 : 2, p.y, p.m, p.n, 32)))
+    return cudaErrorInvalidValue;
+  const int m_tiles = static_cast<int>((p.m + 2 * BM - 1) / (2 * BM)), n_tiles = static_cast<int>((p.n + BN - 1) / BN);
+  const int64_t tiles = static_cast<int64_t>(m_tiles) * n_tiles;
+  const int pairs = static_cast<int>(tiles < p.sms / 2 ? tiles : p.sms / 2);
+  return launch_cluster(kernel, dim3(static_cast<unsigned>(2 * pairs)), kThreads, kSmemBytes, 2, p.stream, ta, tw, ty, p.a_scales,
+                        p.w_scales, p.bias, p.y, static_cast<int>(p.m), static_cast<int>(p.n), p.k_blocks, m_tiles, n_tiles, p.err);
+}
+
+cudaError_t launch_pair(const Product& p) {
+  const bool tma = p.n % (p.f32 ? 4 : 8) == 0;
+  if (p.f32) return tma ? launch_pair_as<true, true>(p) : launch_pair_as<true, false>(p);
+  return tma ? launch_pair_as<false, true>(p) : launch_pair_as<false, false>(p);
+}
+
+template <bool kF32Out, int kRows>
+cudaError_t launch_swap_as(const Product& p, int rows, int row_tiles) {
+  using namespace swap;
+  auto kernel = linear_swap<kF32Out, kRows>;
+  static unsigned long long configured = 0;
+  if (const cudaError_t e = set_smem_once(kernel, static_cast<int>(kSmemBytes), configured); e != cudaSuccess) return e;
+  CUtensorMap ta, tw;
+  if (!make_map(&ta, p.enc, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.a, p.m, p.k, rows) ||
+      !make_map(&tw, p.enc, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.w, p.n, p.k, BN))
+    return cudaErrorInvalidValue;
+  const int64_t n_tiles = (p.n + BN - 1) / BN, tiles = n_tiles * row_tiles;
+  // K's parts: as few blocks of K one after another as the 2 CTAs of every SM allow, a CTA's beginning and end counted
+  // as kEnds blocks.
+  constexpr int kEnds = 6;
+  int parts = 1;
+  int64_t best = 0;
+  for (int c = 1; c <= 8 && c <= p.k_blocks; ++c) {
+    const int64_t waves = (tiles * c + 2 * p.sms - 1) / (2 * p.sms), cost = waves * ((p.k_blocks + c - 1) / c + kEnds);
+    if (c == 1 || cost < best) {
+      best = cost;
+      parts = c;
+    }
+  }
+  int stages = kRingBytes / (kWBytes + rows * kRowBytes);
+  if (stages > kMostStages) stages = kMostStages;
+  return launch_cluster(kernel, dim3(static_cast<unsigned>(n_tiles * parts), static_cast<unsigned>(row_tiles)),
+                        kThreads, kSmemBytes, parts, p.stream, ta, tw, p.a_scales, p.w_scales, p.bias, p.y,
+                        static_cast<int>(p.m), static_cast<int>(p.n), p.k_blocks, rows, stages, p.err);
+}
+
+template <bool kF32Out>
+cudaError_t launch_swap(const Product& p) {
+  const int row_tiles = static_cast<int>((p.m + swap::kMostRows - 1) / swap::kMostRows);
+  const int rows = static_cast<int>(((p.m + row_tiles - 1) / row_tiles + 15) / 16 * 16);
+  return rows <= 16    ? launch_swap_as<kF32Out, 16>(p, rows, row_tiles)
+         : rows <= 32  ? launch_swap_as<kF32Out, 32>(p, rows, row_tiles)
+         : rows <= 64  ? launch_swap_as<kF32Out, 64>(p, rows, row_tiles)
+                       : launch_swap_as<kF32Out, 128>(p, rows, row_tiles);
 }
 
 }  // namespace
@@ -242,26 +761,18 @@ extern "C" int sl_linear_block_fp8(const uint8_t* a, const float* a_scales, cons
                                    const uint16_t* bias, int64_t m, int64_t n, int64_t k, void* y, int y_type,
                                    void* stream) {
   using namespace sl;
-  // Tile coordinates are 32-bit; the grid's second dimension ends at 65535 tiles.
-  if (m < 0 || m > 65535LL * BM || n < 1 || n > 0x7FFFFF00 || k < 16 || k % 16 != 0 || k > 0x7FFFFF00 ||
-      (y_type != SL_BF16 && y_type != SL_F32))
+  // Tile coordinates and tile counts are 32-bit.
+  if (m < 0 || m > 0x7FFFFF00 || n < 1 || n > 0x7FFFFF00 || k < 16 || k % 16 != 0 || k > 0x7FFFFF00 ||
+      (m / 128 + 1) * (n / 128 + 1) > 0x0FFFFFFF || (y_type != SL_BF16 && y_type != SL_F32))
     return SL_INVALID_ARG;
   if (m == 0) return SL_OK;
   for (const void* p : {static_cast<const void*>(a), static_cast<const void*>(w), static_cast<const void*>(y)})
     if (p == nullptr || !aligned(p, 16)) return SL_INVALID_ARG;
   if (a_scales == nullptr || w_scales == nullptr || !aligned(a_scales, 4) || !aligned(w_scales, 4) || !aligned(bias, 2))
     return SL_INVALID_ARG;
-  encode_fn enc = encoder();
-  int* err = error_word();
-  if (enc == nullptr || err == nullptr) return SL_CUDA_ERROR;
-  CUtensorMap ta, tw;
-  if (!make_map(&ta, enc, a, m, k, BM) || !make_map(&tw, enc, w, n, k, BN)) return SL_INVALID_ARG;
-  auto kernel = y_type == SL_F32 ? linear_block_fp8_k<true> : linear_block_fp8_k<false>;
-  if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemBytes));
-      e != cudaSuccess)
-    return status_of(e);
-  const dim3 grid(static_cast<unsigned>((n + BN - 1) / BN), static_cast<unsigned>((m + BM - 1) / BM));
-  return status_of(launch(kernel, grid, dim3(kThreads), kSmemBytes, static_cast<cudaStream_t>(stream), ta, tw, a_scales,
-                          w_scales, bias, y, static_cast<int>(m), static_cast<int>(n),
-                          static_cast<int>((k + BK - 1) / BK), err));
+  const Product p{a, w, a_scales, w_scales, bias, m, n, k, y, y_type == SL_F32, static_cast<int>((k + BK - 1) / BK),
+                  sm_count(), encoder(), error_word(), static_cast<cudaStream_t>(stream)};
+  if (p.enc == nullptr || p.err == nullptr || p.sms < 2) return SL_CUDA_ERROR;
+  if (m <= 2 * swap::kMostRows) return status_of(p.f32 ? launch_swap<true>(p) : launch_swap<false>(p));
+  return status_of(launch_pair(p));
 }
