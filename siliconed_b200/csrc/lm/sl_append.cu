@@ -166,7 +166,7 @@ extern "C" int sl_append_paged(const uint16_t* qkv, int64_t tokens, int heads, i
   const bool e4m3 = cache_type == SL_E4M3;
   if (e4m3 != (k_scale != nullptr) || e4m3 != (v_scale != nullptr) || !aligned(k_scale, 4) || !aligned(v_scale, 4))
     return SL_INVALID_ARG;
-  int* err = error_word();
+  int* const err = current_device().err;
   if (err == nullptr) return SL_CUDA_ERROR;
   const Append a{qkv,       tokens,  heads,  kv_heads, norm_q,      norm_k, freqs,     eps,     max_pos, seq,     positions,
                  table,     seqs,    table_width, pages, page_size, k_cache, v_cache, k_scale, v_scale, q,       err};

@@ -742,16 +742,6 @@ cudaError_t launch_dim(const Attention& a, bool e4m3, int sms, cudaStream_t stre
   return e4m3 ? launch_kind<kDim, true>(a, sms, stream) : launch_kind<kDim, false>(a, sms, stream);
 }
 
-// The SMs of the current device (0: none).
-int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
-    cudaGetLastError();
-    return 0;
-  }
-  return n;
-}
-
 bool shape_ok(int heads, int kv_heads, int head_dim) {
   return heads >= 1 && kv_heads >= 1 && heads <= 65536 && heads % kv_heads == 0 &&
          (head_dim == 64 || head_dim == 128);
@@ -762,17 +752,20 @@ int tile_rows(int heads, int kv_heads) { return heads / kv_heads <= 8 ? 8 : 16; 
 // Counters, rounded up to 16 bytes, then two parts a worker.
 size_t counter_bytes(int workers) { return (static_cast<size_t>(workers) * 4 + 15) / 16 * 16; }
 
+size_t workspace_bytes_of(int sms, int heads, int kv_heads, int head_dim) {
+  const int workers = sms * kMostCtasPerSm;
+  return counter_bytes(workers) + static_cast<size_t>(workers) * 2 * tile_rows(heads, kv_heads) * (head_dim + 2) * sizeof(float);
+}
+
 }  // namespace
 }  // namespace sl
 
 extern "C" int sl_paged_attention_workspace(int heads, int kv_heads, int head_dim, size_t* bytes) {
   using namespace sl;
   if (bytes == nullptr || !shape_ok(heads, kv_heads, head_dim)) return SL_INVALID_ARG;
-  const int sms = sm_count();
+  const int sms = current_device().sms;
   if (sms == 0) return SL_CUDA_ERROR;
-  const int workers = sms * kMostCtasPerSm;
-  *bytes = counter_bytes(workers) +
-           static_cast<size_t>(workers) * 2 * tile_rows(heads, kv_heads) * (head_dim + 2) * sizeof(float);
+  *bytes = workspace_bytes_of(sms, heads, kv_heads, head_dim);
   return SL_OK;
 }
 
@@ -802,12 +795,11 @@ extern "C" int sl_paged_attention(const uint16_t* q, const void* k_cache, const 
   const bool e4m3 = cache_type == SL_E4M3;
   if (e4m3 != (k_scale != nullptr) || e4m3 != (v_scale != nullptr) || !aligned(k_scale, 4) || !aligned(v_scale, 4))
     return SL_INVALID_ARG;
-  size_t need = 0;
-  if (const int s = sl_paged_attention_workspace(heads, kv_heads, head_dim, &need); s != SL_OK) return s;
-  if (workspace_bytes < need) return SL_INVALID_ARG;
-  const int sms = sm_count(), workers = sms * kMostCtasPerSm;
-  int* err = error_word();
-  if (err == nullptr) return SL_CUDA_ERROR;
+  const Device device = current_device();
+  if (device.err == nullptr) return SL_CUDA_ERROR;
+  const int sms = device.sms, workers = sms * kMostCtasPerSm;
+  int* const err = device.err;
+  if (workspace_bytes < workspace_bytes_of(sms, heads, kv_heads, head_dim)) return SL_INVALID_ARG;
   const int group = heads / kv_heads;
   int shift = -1;
   if ((page_size & (page_size - 1)) == 0)

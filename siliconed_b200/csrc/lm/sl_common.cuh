@@ -32,8 +32,12 @@ enum Site : int {
 constexpr float kE4m3Max = 448.0f;
 constexpr float kScaleFloor = 1e-30f;
 
-// The device error word of the current device: [0] the code, [1] the site, [2] the block.
-int* error_word();
+// What a launch needs to know of the current device, asked of the runtime once per device.
+struct Device {
+  int sms;   // its SMs; 0: the runtime gave an error
+  int* err;  // the library's error word: [0] the code, [1] the site, [2] the block
+};
+Device current_device();
 
 inline int status_of(cudaError_t e) {
   if (e == cudaSuccess) return SL_OK;

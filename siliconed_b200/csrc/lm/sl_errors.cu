@@ -1,19 +1,40 @@
-// The library's error word, one per device.
+// The library's error word, one per device, and what is remembered of each device.
+#include <atomic>
+
 #include "sl_common.cuh"
 
 namespace {
 __device__ int g_errors[4];
-}
+
+constexpr int kDevices = 64;
+std::atomic<int> g_sms[kDevices];
+std::atomic<int*> g_words[kDevices];
+}  // namespace
 
 namespace sl {
 
-int* error_word() {
-  void* p = nullptr;
-  if (cudaGetSymbolAddress(&p, g_errors) != cudaSuccess) {
+Device current_device() {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
     cudaGetLastError();
-    return nullptr;
+    return {0, nullptr};
   }
-  return static_cast<int*>(p);
+  if (dev < kDevices) {
+    int* const word = g_words[dev].load(std::memory_order_acquire);
+    if (word != nullptr) return {g_sms[dev].load(std::memory_order_relaxed), word};
+  }
+  int sms = 0;
+  void* word = nullptr;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
+      cudaGetSymbolAddress(&word, g_errors) != cudaSuccess) {
+    cudaGetLastError();
+    return {0, nullptr};
+  }
+  if (dev < kDevices) {
+    g_sms[dev].store(sms, std::memory_order_relaxed);
+    g_words[dev].store(static_cast<int*>(word), std::memory_order_release);
+  }
+  return {sms, static_cast<int*>(word)};
 }
 
 }  // namespace sl

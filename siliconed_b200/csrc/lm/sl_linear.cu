@@ -17,7 +17,7 @@
 //   128 with four buffers: 198 us, their MMAs read shared memory half again as often.  fma.rn.f32x2 for the sums: 293 us,
 //   pairs of registers moved together.  One issuing thread: 212 us.)
 // - linear_swap: for few rows, bound by reading the weight.  The operands change places: 128 weight rows are the MMA's
-//   M and the rows of a, in tiles of up to 128, its N, so that no MMA row or TMEM column is padding; K is cut over the
+//   M and the rows of a, in tiles of up to 64, its N, so that no MMA row or TMEM column is padding; K is cut over the
 //   CTAs of a cluster, whose partials meet through distributed shared memory and are added in rank order.
 //
 // Rows past m or n and values past k arrive as zeros.  Every wait is bounded; no load uses cluster multicast.
@@ -54,7 +54,7 @@ __device__ __forceinline__ void mma_e4m3(uint32_t d_tmem, uint64_t adesc, uint64
 }
 
 // Waits for this thread's TMEM loads; the values it loaded cannot be used above it.
-__device__ __forceinline__ void tmem_wait_32(uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
                  "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
@@ -62,19 +62,21 @@ __device__ __forceinline__ void tmem_wait_32(uint32_t (&r)[32]) {
                  "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
 }
 
-__device__ __forceinline__ uint64_t pair_of(uint32_t lo, uint32_t hi) {
-  uint64_t v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
-  return v;
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
 }
-__device__ __forceinline__ float2 floats_of(uint64_t v) {
-  uint32_t lo, hi;
-  asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(v));
-  return make_float2(__uint_as_float(lo), __uint_as_float(hi));
-}
-// Two fp32 a * b + c, each rounded once.
-__device__ __forceinline__ void fma2(uint64_t& c, uint64_t a, uint64_t b) {
-  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(a), "l"(b));
+// 32 (16) consecutive fp32 columns of this thread's TMEM lane.
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[32]) { sc::tmem_ld_32(taddr, r); }
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
 }
 
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int c0, int c1) {
@@ -196,7 +198,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         a_scale = sa[next];
         w_scale = sw[next];
         uint32_t r[3][32];
-        const auto load = [&](int q, uint32_t(&into)[32]) { sc::tmem_ld_32(lanes + buf * BN + q * 32, into); };
+        const auto load = [&](int q, uint32_t(&into)[32]) { tmem_load(lanes + buf * BN + q * 32, into); };
         const auto add = [&](int q, const uint32_t(&part)[32]) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) acc[q * 32 + j] = fmaf(__uint_as_float(part[j]), f, acc[q * 32 + j]);
@@ -204,12 +206,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         load(0, r[0]);
         load(1, r[1]);
         load(2, r[2]);
-        tmem_wait_32(r[0]);
-        tmem_wait_32(r[1]);
-        tmem_wait_32(r[2]);
+        tmem_wait(r[0]);
+        tmem_wait(r[1]);
+        tmem_wait(r[2]);
         add(0, r[0]);
         load(3, r[0]);
-        tmem_wait_32(r[0]);
+        tmem_wait(r[0]);
         // All of the partial is in registers: its buffer is free.
         sc::tc_fence_before();
         __syncwarp();
@@ -354,25 +356,28 @@ __global__ void __launch_bounds__(kThreads, 1)
 namespace swap {
 
 constexpr int BN = 128;                   // rows of w (columns of y) a CTA
-constexpr int kMostRows = 128;            // rows of a, the MMA's N
+constexpr int kMostRows = 64;            // rows of a, the MMA's N
 constexpr int kWBytes = BN * kRowBytes;
 constexpr int kMostStages = 6;
-constexpr int kRingBytes = 104 * 1024;    // two CTAs an SM
-constexpr int kEpiWarp0 = 2, kEpiWarps = 4, kEpiThreads = kEpiWarps * 32;
+constexpr int kRingBytes = 100 * 1024;    // two CTAs an SM
+constexpr int kGroup = 8;                 // blocks whose factors are brought in together
+constexpr int kBuffers = 4;               // partial products in TMEM
+constexpr int kEpiWarp0 = 3, kEpiWarps = 4, kEpiThreads = kEpiWarps * 32;
 constexpr int kThreads = (kEpiWarp0 + kEpiWarps) * 32;
 
 struct Control {
-  uint64_t full[kMostStages], empty[kMostStages];
-  uint64_t part_full[2], part_empty[2];
-  uint64_t drain;
+  uint64_t full[kMostStages];
+  uint64_t done[kMostStages];             // the stage's MMAs completed: its partial is there, the stage is free
+  uint64_t part_empty[kBuffers];
+  uint64_t drain[2];
   uint32_t tmem_base;
   int abort;
-  float factors[2][kMostRows];            // sa * sw of the block, by its parity
+  alignas(16) float factors[2][kGroup][kMostRows];  // sa * sw of a group of blocks, by the group's parity
 };
 constexpr size_t kSmemBytes = kRingBytes + 1024;
 static_assert(kMostRows * BN * 4 <= kRingBytes, "a partial fits the ring");
 
-// kRows: the sums' registers (16, 32, 64 or 128); `rows` <= kRows is the tile's count, a multiple of 16, and the rows of
+// kRows: the sums' registers (16, 32 or 64); `rows` <= kRows is the tile's count, a multiple of 16, and the rows of
 // a's TMA box.
 template <bool kF32Out, int kRows>
 __global__ void __launch_bounds__(kThreads, 2)
@@ -380,9 +385,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                 const float* __restrict__ a_scales, const float* __restrict__ w_scales,
                 const uint16_t* __restrict__ bias, void* __restrict__ y, int m, int n, int k_blocks, int rows, int stages,
                 int* err) {
-  constexpr int kBuffers = 2;
   constexpr uint32_t kTmemCols = kBuffers * kRows;
-  constexpr int kChunk = kRows < 32 ? 16 : 32;           // TMEM columns of a load
   extern __shared__ uint8_t smem_raw[];
   __shared__ Control s;
   uint8_t* const ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -399,13 +402,10 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (threadIdx.x == 0) {
     for (int i = 0; i < stages; ++i) {
       sc::mbar_init(&s.full[i], 1);
-      sc::mbar_init(&s.empty[i], 1);
+      sc::mbar_init(&s.done[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
-      sc::mbar_init(&s.part_full[i], 1);
-      sc::mbar_init(&s.part_empty[i], kEpiWarps);
-    }
-    sc::mbar_init(&s.drain, 1);
+    for (int i = 0; i < kBuffers; ++i) sc::mbar_init(&s.part_empty[i], kEpiWarps);
+    for (int i = 0; i < 2; ++i) sc::mbar_init(&s.drain[i], 1);
     s.abort = 0;
     sc::fence_mbar_init();
     sc::prefetch_tensormap(&tm_a);
@@ -415,6 +415,13 @@ __global__ void __launch_bounds__(kThreads, 2)
     sc::tmem_alloc(&s.tmem_base, kTmemCols);
     sc::tmem_relinquish();
   }
+  // The weight on its way to L2 while the kernel before this one ends: L2 holds what that kernel writes too, so nothing
+  // stale can come of it.
+  if (warp == kEpiWarp0 && lane == 0)
+    for (int kb = kb0; kb < kb1; ++kb)
+      asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(&tm_w)),
+                   "r"(kb * BK), "r"(n0)
+                   : "memory");
   sc::tc_fence_before();
   __syncthreads();
   sc::tc_fence_after();
@@ -426,7 +433,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       int stage = 0;
       uint32_t phase = 0, issued = 0, last_parity = 0;
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!wait(&s.empty[stage], phase ^ 1u, abort, err, kSiteLinearLoad)) break;
+        if (!wait(&s.done[stage], phase ^ 1u, abort, err, kSiteLinearLoad)) break;
         sc::mbar_arrive_expect_tx(&s.full[stage], stage_bytes);
         sc::tma_load_2d(ring + stage * stage_bytes, &tm_w, &s.full[stage], kb * BK, n0);
         sc::tma_load_2d(ring + stage * stage_bytes + kWBytes, &tm_a, &s.full[stage], kb * BK, m0);
@@ -440,14 +447,16 @@ __global__ void __launch_bounds__(kThreads, 2)
       for (int st = 0; st < stages; ++st)
         if (issued & (1u << st)) sc::mbar_wait_drain(&s.full[st], (last_parity >> st) & 1u);
     }
-  } else if (warp == 1) {
+  } else if (warp < kEpiWarp0) {
+    // Two threads issue the MMAs, block by block in turns: a block costs its thread some 770 cycles of issue, commit and
+    // waits, its MMAs 64 to 256.
     if (lane == 0) {
       const uint32_t idesc = idesc_e4m3(BN, rows);
-      int stage = 0, buf = 0;
-      uint32_t phase = 0, buf_phase = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!wait(&s.part_empty[buf], buf_phase ^ 1u, abort, err, kSiteLinearBuffer) ||
-            !wait(&s.full[stage], phase, abort, err, kSiteLinearMma))
+      const int turn = warp - 1;
+      for (int g = turn; g < kb1 - kb0; g += 2) {
+        const int buf = g % kBuffers, stage = g % stages;
+        if (!wait(&s.part_empty[buf], (g / kBuffers & 1) ^ 1u, abort, err, kSiteLinearBuffer) ||
+            !wait(&s.full[stage], g / stages & 1, abort, err, kSiteLinearMma))
           break;
         sc::tc_fence_after();
         const uint32_t w0 = sc::smem_u32(ring + stage * stage_bytes), a0 = w0 + kWBytes;
@@ -455,83 +464,77 @@ __global__ void __launch_bounds__(kThreads, 2)
         for (int kk = 0; kk < BK / 32; ++kk)
           mma_e4m3<false>(tmem + static_cast<uint32_t>(buf * kRows), sc::umma_desc_sw128(w0 + kk * 32),
                           sc::umma_desc_sw128(a0 + kk * 32), idesc, kk != 0 ? 1u : 0u);
-        sc::tc_commit(&s.empty[stage]);
-        sc::tc_commit(&s.part_full[buf]);
-        if (++stage == stages) {
-          stage = 0;
-          phase ^= 1u;
-        }
-        if (++buf == kBuffers) {
-          buf = 0;
-          buf_phase ^= 1u;
-        }
+        sc::tc_commit(&s.done[stage]);
       }
-      sc::tc_commit(&s.drain);
-      sc::mbar_wait_drain(&s.drain, 0);
+      sc::tc_commit(&s.drain[turn]);
+      sc::mbar_wait_drain(&s.drain[turn], 0);
     }
   } else {
-    // One column of y a thread; the block's factors sa * sw come through shared memory, a block ahead of their use.
+    // One column of y a thread.  The factors sa * sw come through shared memory, a group of blocks ahead of their use:
+    // thread t brings those of row t, lane i the weight's scale of block i.
     const int et = threadIdx.x - kEpiWarp0 * 32, quarter = warp & 3;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     const float* sw = w_scales + static_cast<int64_t>(tile) * k_blocks;
     const bool owns = et < rows && m0 + et < m;
     const float* sa = a_scales + static_cast<int64_t>(owns ? m0 + et : 0) * k_blocks;
-    uint64_t acc[kRows / 2];
+    float acc[kRows], a_next[kGroup], w_next;
 #pragma unroll
-    for (int j = 0; j < kRows / 2; ++j) acc[j] = 0;
-    // Sums of the partial of every block; a wait that gave up leaves the sums as they are, but the loop goes on, so
-    // that every warp meets the others at each block's barrier.
-    // The scales are asked for two blocks ahead, into registers of their own for even and odd blocks.
-    const auto scale_at = [&](const float* p, int kb) { return owns && kb < kb1 ? p[kb] : 0.0f; };
-    float a_even = scale_at(sa, kb0), w_even = scale_at(sw, kb0), a_odd = scale_at(sa, kb0 + 1), w_odd = scale_at(sw, kb0 + 1);
-    int buf = 0;
+    for (int j = 0; j < kRows; ++j) acc[j] = 0.0f;
+    const auto ask = [&](int kb) {
+#pragma unroll
+      for (int i = 0; i < kGroup; ++i) a_next[i] = owns && kb + i < kb1 ? sa[kb + i] : 0.0f;
+      w_next = lane < kGroup && kb + lane < kb1 ? sw[kb + lane] : 0.0f;
+    };
+    ask(kb0);
+    int buf = 0, stage = 0;
     uint32_t phase = 0;
-    const auto add_block = [&](int kb, float& a_scale, float& w_scale) {
-      if (et < kRows) s.factors[kb & 1][et] = a_scale * w_scale;
-      a_scale = scale_at(sa, kb + 2);
-      w_scale = scale_at(sw, kb + 2);
-      sc::named_barrier_sync(1, kEpiThreads);
-      const float* f = s.factors[kb & 1];
-      const bool ok = wait_warp(&s.part_full[buf], phase, abort, err, kSiteLinearSum);
+    // A wait that gave up leaves the sums as they are, but the loop goes on, so that every warp meets the others at each
+    // group's barrier.
+    for (int kb = kb0; kb < kb1; ++kb) {
+      const int in_group = (kb - kb0) % kGroup;
+      float(*factors)[kMostRows] = s.factors[(kb - kb0) / kGroup & 1];
+      if (in_group == 0) {
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i) {
+          const float f = a_next[i] * __shfl_sync(0xFFFFFFFFu, w_next, i);
+          if (et < kRows) factors[i][et] = f;
+        }
+        ask(kb + kGroup);
+        sc::named_barrier_sync(1, kEpiThreads);
+      }
+      const float4* f = reinterpret_cast<const float4*>(factors[in_group]);
+      const bool ok = wait_warp(&s.done[stage], phase, abort, err, kSiteLinearSum);
       sc::tc_fence_after();
       if (ok) {
+        constexpr int kChunk = kRows == 32 ? 32 : 16;  // 64 rows: the registers take no more
 #pragma unroll
-        for (int q = 0; q < kRows / kChunk; ++q) {
-          if (q * kChunk >= rows) break;
-          uint32_t r[32];
-          if (kChunk == 32) {
-            sc::tmem_ld_32(lanes + buf * kRows + q * 32, r);
-          } else {
-            asm volatile(
-                "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-                "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-                  "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-                : "r"(lanes + buf * kRows + q * 16)
-                : "memory");
+        for (int q = 0; q < kRows; q += kChunk) {
+          if (q >= rows) break;
+          uint32_t r[kChunk];
+          tmem_load(lanes + buf * kRows + q, r);
+          float4 v[kChunk / 4];
 #pragma unroll
-            for (int j = 16; j < 32; ++j) r[j] = 0;
+          for (int j = 0; j < kChunk / 4; ++j) v[j] = f[q / 4 + j];
+          tmem_wait(r);
+          if (q + kChunk >= rows) {  // all of the partial is in registers: its buffer is free
+            sc::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) sc::mbar_arrive(&s.part_empty[buf]);
           }
-          tmem_wait_32(r);
 #pragma unroll
           for (int j = 0; j < kChunk; j += 4) {
-            const float4 fv = *reinterpret_cast<const float4*>(f + q * kChunk + j);
-            fma2(acc[(q * kChunk + j) / 2], pair_of(r[j], r[j + 1]), pair_of(__float_as_uint(fv.x), __float_as_uint(fv.y)));
-            fma2(acc[(q * kChunk + j) / 2 + 1], pair_of(r[j + 2], r[j + 3]), pair_of(__float_as_uint(fv.z), __float_as_uint(fv.w)));
+            acc[q + j] = fmaf(__uint_as_float(r[j]), v[j / 4].x, acc[q + j]);
+            acc[q + j + 1] = fmaf(__uint_as_float(r[j + 1]), v[j / 4].y, acc[q + j + 1]);
+            acc[q + j + 2] = fmaf(__uint_as_float(r[j + 2]), v[j / 4].z, acc[q + j + 2]);
+            acc[q + j + 3] = fmaf(__uint_as_float(r[j + 3]), v[j / 4].w, acc[q + j + 3]);
           }
         }
       }
-      sc::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) sc::mbar_arrive(&s.part_empty[buf]);
-      if (++buf == kBuffers) {
-        buf = 0;
+      buf = buf + 1 == kBuffers ? 0 : buf + 1;
+      if (++stage == stages) {
+        stage = 0;
         phase ^= 1u;
       }
-    };
-    for (int kb = kb0; kb < kb1; kb += 2) {
-      add_block(kb, a_even, w_even);
-      if (kb + 1 < kb1) add_block(kb + 1, a_odd, w_odd);
     }
     const int col = quarter * 32 + lane;
     if (parts == 1) {
@@ -540,8 +543,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
         for (int j = 0; j < kRows; ++j)
           if (j < rows && m0 + j < m) {
-            const float2 p = floats_of(acc[j / 2]);
-            const float v = (j & 1 ? p.y : p.x) + add;
+            const float v = acc[j] + add;
             const int64_t at = static_cast<int64_t>(m0 + j) * n + n0 + col;
             if (kF32Out)
               static_cast<float*>(y)[at] = v;
@@ -555,10 +557,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       float* part = reinterpret_cast<float*>(ring);
 #pragma unroll
       for (int j = 0; j < kRows; ++j)
-        if (j < rows) {
-          const float2 p = floats_of(acc[j / 2]);
-          part[j * BN + col] = j & 1 ? p.y : p.x;
-        }
+        if (j < rows) part[j * BN + col] = acc[j];
     }
   }
   __syncwarp();
@@ -640,15 +639,6 @@ bool make_map(CUtensorMap* map, encode_fn enc, CUtensorMapDataType type, int siz
   const cuuint32_t estr[2] = {1, 1};
   return enc(map, type, 2, const_cast<void*>(base), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
-    cudaGetLastError();
-    return 0;
-  }
-  return n;
 }
 
 struct Product {
@@ -750,8 +740,7 @@ cudaError_t launch_swap(const Product& p) {
   const int rows = static_cast<int>(((p.m + row_tiles - 1) / row_tiles + 15) / 16 * 16);
   return rows <= 16    ? launch_swap_as<kF32Out, 16>(p, rows, row_tiles)
          : rows <= 32  ? launch_swap_as<kF32Out, 32>(p, rows, row_tiles)
-         : rows <= 64  ? launch_swap_as<kF32Out, 64>(p, rows, row_tiles)
-                       : launch_swap_as<kF32Out, 128>(p, rows, row_tiles);
+                       : launch_swap_as<kF32Out, 64>(p, rows, row_tiles);
 }
 
 }  // namespace
@@ -770,9 +759,10 @@ extern "C" int sl_linear_block_fp8(const uint8_t* a, const float* a_scales, cons
     if (p == nullptr || !aligned(p, 16)) return SL_INVALID_ARG;
   if (a_scales == nullptr || w_scales == nullptr || !aligned(a_scales, 4) || !aligned(w_scales, 4) || !aligned(bias, 2))
     return SL_INVALID_ARG;
+  const Device device = current_device();
   const Product p{a, w, a_scales, w_scales, bias, m, n, k, y, y_type == SL_F32, static_cast<int>((k + BK - 1) / BK),
-                  sm_count(), encoder(), error_word(), static_cast<cudaStream_t>(stream)};
+                  device.sms, encoder(), device.err, static_cast<cudaStream_t>(stream)};
   if (p.enc == nullptr || p.err == nullptr || p.sms < 2) return SL_CUDA_ERROR;
-  if (m <= 2 * swap::kMostRows) return status_of(p.f32 ? launch_swap<true>(p) : launch_swap<false>(p));
+  if (m <= 3 * swap::kMostRows) return status_of(p.f32 ? launch_swap<true>(p) : launch_swap<false>(p));
   return status_of(launch_pair(p));
 }

@@ -35,7 +35,6 @@ SIGNATURES = {
 }
 
 _lib = None
-_TYPES = {torch.bfloat16: BF16, torch.float32: F32, torch.float8_e4m3fn: E4M3}
 
 
 class LmError(RuntimeError):
@@ -72,40 +71,42 @@ def _check(status: int, what: str) -> None:
         raise LmError(f"{what}: status {status}", status)
 
 
-def _need(what: str, ok: bool, message: str) -> None:
-    if not ok:
-        raise LmError(f"{what}: {message}")
+def _refuse(what: str, name: str, t, dtypes, shape, index: int):
+    got = f"{t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else repr(t)
+    want = " or ".join(str(d).replace("torch.", "") for d in dtypes)
+    size = ", ".join("*" if w is None else str(w) for w in shape)
+    raise LmError(f"{what}: {name} must be a contiguous {want} [{size}] tensor on cuda:{index}: got {got}")
 
 
-def _take(what: str, name: str, t, device, dtypes, shape):
-    """The tensor's address, after its device, dtype, shape (None: any size) and contiguity."""
-    if not isinstance(t, torch.Tensor) or t.dtype not in dtypes or t.dim() != len(shape) or \
-            any(w is not None and w != s for w, s in zip(shape, t.shape)) or not t.is_contiguous() or t.device != device:
-        got = f"{t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else repr(t)
-        want = " or ".join(str(d).replace("torch.", "") for d in dtypes)
-        size = ", ".join("*" if w is None else str(w) for w in shape)
-        raise LmError(f"{what}: {name} must be a contiguous {want} [{size}] tensor on {device}: got {got}")
+def _take(what: str, name: str, t, dtype, shape, index: int) -> int:
+    """The tensor's address, after its dtype, shape, contiguity and device.  (Called for every operand of every call: the
+    message is made only on the way out.)"""
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.shape != shape or t.get_device() != index or \
+            not t.is_contiguous():
+        _refuse(what, name, t, (dtype,), shape, index)
     return t.data_ptr()
 
 
-def _device(what: str, name: str, t):
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise LmError(f"{what}: {name} must be a CUDA tensor")
-    return t.device
+def _index(what: str, name: str, t, dims: int) -> int:
+    """The device index of the operand that names the call's device."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dim() != dims:
+        raise LmError(f"{what}: {name} must be a CUDA tensor of {dims} dimensions")
+    return t.get_device()
 
 
-def _call(fn: str, device, *args) -> None:
-    """The call on `device` and its current stream."""
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if device.index == torch.cuda.current_device():
-        _check(getattr(load(), fn)(*args, stream), fn)
+def _call(fn: str, index: int, *args) -> None:
+    """The call on device `index` and its current stream."""
+    call = getattr(_lib or load(), fn)
+    if index == torch._C._cuda_getDevice():
+        status = call(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(device):
-            _check(getattr(load(), fn)(*args, stream), fn)
+        with torch.cuda.device(index):
+            status = call(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status != OK:
+        raise LmError(f"{fn}: status {status}", status)
 
 
-_BF16, _F32, _I32, _E4M3, _FLOATS = (torch.bfloat16,), (torch.float32,), (torch.int32,), (torch.float8_e4m3fn,), \
-    (torch.bfloat16, torch.float32)
+_BF16, _F32, _I32, _E4M3 = torch.bfloat16, torch.float32, torch.int32, torch.float8_e4m3fn
 
 
 def rms_norm_quantize(x, delta=None, weight=None, eps: float = 1e-6, x_out=None, codes=None, scales=None,
@@ -116,44 +117,51 @@ def rms_norm_quantize(x, delta=None, weight=None, eps: float = 1e-6, x_out=None,
     [rows, ceil(d / 128)]).  ``norm=False`` quantizes z * weight itself.  Without ``delta`` x is not written.
     """
     what = "rms_norm_quantize"
-    device = _device(what, "x", x)
-    _need(what, x.dim() == 2, "x must be [rows, d]")
-    rows, d = x.shape
-    _need(what, d % 16 == 0 and 16 <= d <= 16384, f"d must be a multiple of 16 up to 16384: got {d}")
-    blocks = -(-d // BLOCK)
-    px = _take(what, "x", x, device, _FLOATS, (rows, d))
+    index = _index(what, "x", x, 2)
+    shape = x.shape
+    rows, d = shape
+    if d % 16 != 0 or d < 16 or d > 16384:
+        raise LmError(f"{what}: d must be a multiple of 16 up to 16384: got {d}")
+    blocks = (rows, (d + BLOCK - 1) // BLOCK)
+    if x.dtype is not _F32 and x.dtype is not _BF16:
+        _refuse(what, "x", x, (_BF16, _F32), shape, index)
+    px = po = _take(what, "x", x, x.dtype, shape, index)
     pd = pw = None
+    kind = BF16
     if delta is not None:
-        pd = _take(what, "delta", delta, device, _FLOATS, (rows, d))
+        kind = F32 if getattr(delta, "dtype", None) is _F32 else BF16
+        pd = _take(what, "delta", delta, _F32 if kind == F32 else _BF16, shape, index)
+        if x_out is not None:
+            po = _take(what, "x_out", x_out, x.dtype, shape, index)
+    elif x_out is not None and x_out is not x:
+        raise LmError(f"{what}: x_out without delta must be x")
     if weight is not None:
-        pw = _take(what, "weight", weight, device, _F32, (d,))
-    if x_out is None:
-        x_out = x
-    _need(what, delta is not None or x_out is x, "x_out without delta must be x")
-    po = _take(what, "x_out", x_out, device, (x.dtype,), (rows, d))
+        pw = _take(what, "weight", weight, _F32, (d,), index)
     if codes is None:
-        codes = torch.empty(rows, d, dtype=torch.float8_e4m3fn, device=device)
+        codes = torch.empty(rows, d, dtype=_E4M3, device=x.device)
     if scales is None:
-        scales = torch.empty(rows, blocks, device=device)
-    _call("sl_rms_norm_quantize", device, px, _TYPES[x.dtype], pd, BF16 if delta is None else _TYPES[delta.dtype], pw, eps,
-          int(norm), rows, d, po, _take(what, "codes", codes, device, _E4M3, (rows, d)),
-          _take(what, "scales", scales, device, _F32, (rows, blocks)))
-    return x_out, codes, scales
+        scales = torch.empty(blocks, device=x.device)
+    _call("sl_rms_norm_quantize", index, px, F32 if x.dtype is _F32 else BF16, pd, kind, pw, eps, int(norm), rows, d, po,
+          _take(what, "codes", codes, _E4M3, shape, index), _take(what, "scales", scales, _F32, blocks, index))
+    return x if x_out is None else x_out, codes, scales
 
 
-def _cache(what, k_cache, v_cache, k_scale, v_scale, device, kv_heads, head_dim):
+def _cache(what, k_cache, v_cache, k_scale, v_scale, index, kv_heads, head_dim):
     """(type, pages, page size, the four addresses) of a paged cache."""
-    _need(what, isinstance(k_cache, torch.Tensor) and k_cache.dim() == 4,
-          "k_cache must be [pages, kv_heads, page_size, head_dim]")
+    if not isinstance(k_cache, torch.Tensor) or k_cache.dim() != 4:
+        raise LmError(f"{what}: k_cache must be [pages, kv_heads, page_size, head_dim]")
     pages, _, size, _ = k_cache.shape
     shape = (pages, kv_heads, size, head_dim)
-    pk = _take(what, "k_cache", k_cache, device, _BF16 + _E4M3, shape)
-    pv = _take(what, "v_cache", v_cache, device, (k_cache.dtype,), shape)
-    if k_cache.dtype == torch.bfloat16:
-        _need(what, k_scale is None and v_scale is None, "a bf16 cache has no scales")
-        return BF16, pages, size, pk, pv, None, None
-    return E4M3, pages, size, pk, pv, _take(what, "k_scale", k_scale, device, _F32, shape[:3]), \
-        _take(what, "v_scale", v_scale, device, _F32, shape[:3])
+    if pages == 0 or size == 0:
+        raise LmError(f"{what}: an empty cache")
+    if k_cache.dtype is _BF16:
+        if k_scale is not None or v_scale is not None:
+            raise LmError(f"{what}: a bf16 cache has no scales")
+        return BF16, pages, size, _take(what, "k_cache", k_cache, _BF16, shape, index), \
+            _take(what, "v_cache", v_cache, _BF16, shape, index), None, None
+    return E4M3, pages, size, _take(what, "k_cache", k_cache, _E4M3, shape, index), \
+        _take(what, "v_cache", v_cache, _E4M3, shape, index), _take(what, "k_scale", k_scale, _F32, shape[:3], index), \
+        _take(what, "v_scale", v_scale, _F32, shape[:3], index)
 
 
 def append_paged(qkv, heads: int, kv_heads: int, norm_q, norm_k, eps: float, freqs, pairs: str, seq, positions, table,
@@ -166,26 +174,31 @@ def append_paged(qkv, heads: int, kv_heads: int, norm_q, norm_k, eps: float, fre
     head_dim], bf16, or float8_e4m3fn with fp32 scales [pages, kv_heads, page_size].
     """
     what = "append_paged"
-    device = _device(what, "qkv", qkv)
-    _need(what, heads >= 1 and kv_heads >= 1, "heads and kv_heads must be positive")
-    _need(what, qkv.dim() == 2 and qkv.shape[1] % (heads + 2 * kv_heads) == 0, "qkv must be [tokens, (heads + 2 kv_heads) * head_dim]")
+    index = _index(what, "qkv", qkv, 2)
+    if heads < 1 or kv_heads < 1 or qkv.shape[1] % (heads + 2 * kv_heads) != 0:
+        raise LmError(f"{what}: qkv must be [tokens, (heads + 2 kv_heads) * head_dim]")
     tokens, dim = qkv.shape[0], qkv.shape[1] // (heads + 2 * kv_heads)
-    _need(what, dim in (64, 128), f"head_dim must be 64 or 128: got {dim}")
-    _need(what, pairs in PAIRS, f"pairs must be one of {sorted(PAIRS)}: got {pairs!r}")
-    kind, pages, size, pk, pv, pks, pvs = _cache(what, k_cache, v_cache, k_scale, v_scale, device, kv_heads, dim)
-    pf = _take(what, "freqs", freqs, device, _F32, (None, dim // 2, 2))
-    pt = _take(what, "table", table, device, _I32, (None, None))
-    seqs, width = table.shape
-    _need(what, freqs.shape[0] > 0 and seqs > 0 and width > 0 and pages > 0 and size > 0, "an empty table, cache or freqs")
-    _need(what, seq is not None or tokens <= seqs, f"{tokens} tokens for {seqs} sequences")
+    if dim != 128 and dim != 64:
+        raise LmError(f"{what}: head_dim must be 64 or 128: got {dim}")
+    if pairs not in PAIRS:
+        raise LmError(f"{what}: pairs must be one of {sorted(PAIRS)}: got {pairs!r}")
+    kind, pages, size, pk, pv, pks, pvs = _cache(what, k_cache, v_cache, k_scale, v_scale, index, kv_heads, dim)
+    if not isinstance(freqs, torch.Tensor) or freqs.dim() != 3 or not isinstance(table, torch.Tensor) or table.dim() != 2:
+        raise LmError(f"{what}: freqs must be [max_pos, head_dim / 2, 2], table [seqs, width]")
+    max_pos, (seqs, width) = freqs.shape[0], table.shape
+    if max_pos == 0 or seqs == 0 or width == 0:
+        raise LmError(f"{what}: an empty table or freqs")
+    if seq is None and tokens > seqs:
+        raise LmError(f"{what}: {tokens} tokens for {seqs} sequences")
     if q is None:
-        q = torch.empty(tokens, heads, dim, dtype=torch.bfloat16, device=device)
-    _call("sl_append_paged", device, _take(what, "qkv", qkv, device, _BF16, (tokens, None)), tokens, heads, kv_heads, dim,
-          None if norm_q is None else _take(what, "norm_q", norm_q, device, _F32, (dim,)),
-          None if norm_k is None else _take(what, "norm_k", norm_k, device, _F32, (dim,)), eps, pf, freqs.shape[0],
-          PAIRS[pairs], None if seq is None else _take(what, "seq", seq, device, _I32, (tokens,)),
-          _take(what, "positions", positions, device, _I32, (tokens,)), pt, seqs, width, pages, size, kind, pk, pv, pks, pvs,
-          _take(what, "q", q, device, _BF16, (tokens, heads, dim)))
+        q = torch.empty(tokens, heads, dim, dtype=_BF16, device=qkv.device)
+    _call("sl_append_paged", index, _take(what, "qkv", qkv, _BF16, qkv.shape, index), tokens, heads, kv_heads, dim,
+          None if norm_q is None else _take(what, "norm_q", norm_q, _F32, (dim,), index),
+          None if norm_k is None else _take(what, "norm_k", norm_k, _F32, (dim,), index), eps,
+          _take(what, "freqs", freqs, _F32, (max_pos, dim // 2, 2), index), max_pos, PAIRS[pairs],
+          None if seq is None else _take(what, "seq", seq, _I32, (tokens,), index),
+          _take(what, "positions", positions, _I32, (tokens,), index), _take(what, "table", table, _I32, (seqs, width), index),
+          seqs, width, pages, size, kind, pk, pv, pks, pvs, _take(what, "q", q, _BF16, (tokens, heads, dim), index))
     return q
 
 
@@ -194,7 +207,8 @@ _workspaces: dict = {}
 
 def attention_workspace(heads: int, kv_heads: int, head_dim: int, device=None):
     """A zeroed workspace for ``paged_attention``: one per stream whose calls may run at the same time."""
-    device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    device = torch.device("cuda", torch.cuda.current_device() if device is None else device) \
+        if device is None or isinstance(device, int) else torch.device(device)
     need = _SZ()
     with torch.cuda.device(device):
         _check(load().sl_paged_attention_workspace(heads, kv_heads, head_dim, ctypes.byref(need)),
@@ -202,15 +216,15 @@ def attention_workspace(heads: int, kv_heads: int, head_dim: int, device=None):
         return torch.zeros(need.value, dtype=torch.uint8, device=device)
 
 
-def _stream_workspace(heads, kv_heads, dim, device):
+def _stream_workspace(heads, kv_heads, dim, index):
     """The current stream's workspace.  A call under graph capture gets one of its own, zeroed inside the graph: memory
     that only a replay writes must not be handed to later calls."""
     if torch.cuda.is_current_stream_capturing():
-        return attention_workspace(heads, kv_heads, dim, device)
-    key = (device.index, torch.cuda.current_stream(device).cuda_stream, heads // kv_heads > 8, dim)
+        return attention_workspace(heads, kv_heads, dim, index)
+    key = (index, torch._C._cuda_getCurrentRawStream(index), heads > 8 * kv_heads, dim)
     ws = _workspaces.get(key)
     if ws is None:
-        ws = _workspaces[key] = attention_workspace(heads, kv_heads, dim, device)
+        ws = _workspaces[key] = attention_workspace(heads, kv_heads, dim, index)
     return ws
 
 
@@ -222,26 +236,28 @@ def paged_attention(q, k_cache, v_cache, k_scale, v_scale, table, lengths, scale
     given) is filled with log sum exp.  A sequence of length 0 gives zeros and -inf.
     """
     what = "paged_attention"
-    device = _device(what, "q", q)
-    _need(what, q.dim() == 3, "q must be [batch, heads, head_dim]")
-    batch, heads, dim = q.shape
-    _need(what, dim in (64, 128), f"head_dim must be 64 or 128: got {dim}")
-    _need(what, isinstance(k_cache, torch.Tensor) and k_cache.dim() == 4, "k_cache must be [pages, kv_heads, page_size, head_dim]")
-    kv_heads = k_cache.shape[1]
-    _need(what, kv_heads > 0 and heads > 0 and heads % kv_heads == 0, f"{kv_heads} key-value heads for {heads} query heads")
-    kind, pages, size, pk, pv, pks, pvs = _cache(what, k_cache, v_cache, k_scale, v_scale, device, kv_heads, dim)
-    pt = _take(what, "table", table, device, _I32, (batch, None))
+    index = _index(what, "q", q, 3)
+    shape = q.shape
+    batch, heads, dim = shape
+    if dim != 128 and dim != 64:
+        raise LmError(f"{what}: head_dim must be 64 or 128: got {dim}")
+    kv_heads = k_cache.shape[1] if isinstance(k_cache, torch.Tensor) and k_cache.dim() == 4 else 0
+    if kv_heads < 1 or heads < 1 or heads % kv_heads != 0:
+        raise LmError(f"{what}: {kv_heads} key-value heads for {heads} query heads")
+    kind, pages, size, pk, pv, pks, pvs = _cache(what, k_cache, v_cache, k_scale, v_scale, index, kv_heads, dim)
+    if not isinstance(table, torch.Tensor) or table.dim() != 2 or table.shape[1] == 0:
+        raise LmError(f"{what}: table must be [batch, width]")
     width = table.shape[1]
-    _need(what, width > 0 and pages > 0 and size > 0, "an empty table or cache")
     if out is None:
         out = torch.empty_like(q)
     if workspace is None:
-        workspace = _stream_workspace(heads, kv_heads, dim, device)
-    _call("sl_paged_attention", device, _take(what, "q", q, device, _BF16, (batch, heads, dim)), pk, pv, pks, pvs, kind, pt,
-          _take(what, "lengths", lengths, device, _I32, (batch,)), batch, heads, kv_heads, dim, width, pages, size, scale,
-          _take(what, "out", out, device, _BF16, (batch, heads, dim)),
-          None if lse is None else _take(what, "lse", lse, device, _F32, (batch, heads)),
-          _take(what, "workspace", workspace, device, (torch.uint8,), (None,)), workspace.numel())
+        workspace = _stream_workspace(heads, kv_heads, dim, index)
+    space = workspace.numel()
+    _call("sl_paged_attention", index, _take(what, "q", q, _BF16, shape, index), pk, pv, pks, pvs, kind,
+          _take(what, "table", table, _I32, (batch, width), index), _take(what, "lengths", lengths, _I32, (batch,), index),
+          batch, heads, kv_heads, dim, width, pages, size, scale, _take(what, "out", out, _BF16, shape, index),
+          None if lse is None else _take(what, "lse", lse, _F32, (batch, heads), index),
+          _take(what, "workspace", workspace, torch.uint8, (space,), index), space)
     return out
 
 
@@ -252,18 +268,20 @@ def linear_block_fp8(codes, scales, weight, weight_scales, bias=None, out=None):
     as published, weight_scales fp32 [ceil(n / 128), ceil(k / 128)]; bias: bf16 [n]; out: bf16 (default) or fp32 [m, n].
     """
     what = "linear_block_fp8"
-    device = _device(what, "codes", codes)
-    _need(what, codes.dim() == 2 and isinstance(weight, torch.Tensor) and weight.dim() == 2, "codes must be [m, k], weight [n, k]")
-    (m, k), n = codes.shape, weight.shape[0]
-    _need(what, k >= 16 and k % 16 == 0 and n > 0, f"k must be a multiple of 16 and n positive: got k {k}, n {n}")
-    kb, nb = -(-k // BLOCK), -(-n // BLOCK)
+    index = _index(what, "codes", codes, 2)
+    m, k = codes.shape
+    n = weight.shape[0] if isinstance(weight, torch.Tensor) and weight.dim() == 2 else 0
+    if k < 16 or k % 16 != 0 or n < 1:
+        raise LmError(f"{what}: codes must be [m, k], weight [n, k], k a multiple of 16: got k {k}, n {n}")
+    kb, nb = (k + BLOCK - 1) // BLOCK, (n + BLOCK - 1) // BLOCK
     if out is None:
-        out = torch.empty(m, n, dtype=torch.bfloat16, device=device)
-    _call("sl_linear_block_fp8", device, _take(what, "codes", codes, device, _E4M3, (m, k)),
-          _take(what, "scales", scales, device, _F32, (m, kb)), _take(what, "weight", weight, device, _E4M3, (n, k)),
-          _take(what, "weight_scales", weight_scales, device, _F32, (nb, kb)),
-          None if bias is None else _take(what, "bias", bias, device, _BF16, (n,)), m, n, k,
-          _take(what, "out", out, device, _FLOATS, (m, n)), _TYPES[out.dtype])
+        out = torch.empty(m, n, dtype=_BF16, device=codes.device)
+    kind = F32 if getattr(out, "dtype", None) is _F32 else BF16
+    _call("sl_linear_block_fp8", index, _take(what, "codes", codes, _E4M3, (m, k), index),
+          _take(what, "scales", scales, _F32, (m, kb), index), _take(what, "weight", weight, _E4M3, (n, k), index),
+          _take(what, "weight_scales", weight_scales, _F32, (nb, kb), index),
+          None if bias is None else _take(what, "bias", bias, _BF16, (n,), index), m, n, k,
+          _take(what, "out", out, _F32 if kind == F32 else _BF16, (m, n), index), kind)
     return out
 
 
