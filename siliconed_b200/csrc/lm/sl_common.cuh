@@ -145,14 +145,17 @@ __device__ __forceinline__ uint32_t abs_max8(const float (&v)[8]) {
   return m;
 }
 
-// The scale of values whose largest magnitude has the bits `m`: max(m / 448, 1e-30), a NaN or infinity as it is.
+// The scale of values whose largest magnitude has the bits `m`: max(m / 448, 1e-30), a NaN or infinity as it is.  The
+// quotient by the constant is a product with its reciprocal (an ulp of fp32; the division would be 20 instructions).
 __device__ __forceinline__ float scale_of(uint32_t m) {
-  return m >= 0x7F800000u ? __uint_as_float(m) : fmaxf(__fdiv_rn(__uint_as_float(m), kE4m3Max), kScaleFloor);
+  return m >= 0x7F800000u ? __uint_as_float(m) : fmaxf(__uint_as_float(m) * (1.0f / kE4m3Max), kScaleFloor);
 }
 
-// Eight codes e4m3(v / s).  s is at least 1e-30 and at most 7.6e35, so 1 / s neither overflows nor is subnormal.
+// Eight codes e4m3(v / s), by the reciprocal of s (an ulp of fp32).  s is at least 1e-30 and at most 7.6e35, so the
+// reciprocal neither overflows nor is subnormal; a product past 448 by an ulp is clipped to it.
 __device__ __forceinline__ uint2 quantize8(const float (&v)[8], float s) {
-  const float r = __frcp_rn(s);
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
   return make_uint2(e4m3x2(v[0] * r, v[1] * r) | (e4m3x2(v[2] * r, v[3] * r) << 16),
                     e4m3x2(v[4] * r, v[5] * r) | (e4m3x2(v[6] * r, v[7] * r) << 16));
 }
