@@ -6,7 +6,7 @@
 // block's partial product in TMEM (tcgen05.mma kind::f8f6f4, four MMAs of K 32), and the epilogue warps multiply it
 // by its scales and add it to fp32 sums in registers while the MMAs of the next block run into the other TMEM buffer.
 //
-// Two kernels, by the count of rows (choose()):
+// Two kernels, by their estimated times (swap_plan(), pair_us()):
 //
 // - linear_pair: a cluster of two CTAs owns tiles of 256 x 256 of y (tcgen05.mma.cta_group::2), persistent over the
 //   tiles.  Each CTA loads its own 128 rows of a and of w by TMA (128-byte swizzle).  The tile leaves through shared
@@ -21,6 +21,9 @@
 //   CTAs of a cluster, whose partials meet through distributed shared memory and are added in rank order.
 //
 // Rows past m or n and values past k arrive as zeros.  Every wait is bounded; no load uses cluster multicast.
+#include <atomic>
+#include <cmath>
+
 #include "sl_common.cuh"
 
 namespace sl {
@@ -704,6 +707,75 @@ cudaError_t launch_pair(const Product& p) {
   return tma ? launch_pair_as<false, true>(p) : launch_pair_as<false, false>(p);
 }
 
+// Estimated microseconds (B200, fitted to [m, 2560] x [2560, 9728], [m, 4096] x [4096, 12288 or 4096] and [m, 9728] x
+// [9728, 2560], m 1 to 1024; most within 20 %).  The few-rows kernel: waves of two CTAs an SM, a beginning and an end
+// each, and blocks one after another, slower where a cluster shares K.  The many-rows kernel: a tile's blocks one after
+// another.
+// How many CTAs of the few-rows kernel run at once in clusters of `c` (its instances differ in nothing that matters to that).
+// A cluster lies in one group of SMs, so some sizes leave slots empty: 288 CTAs in clusters of 3 took a second wave, in
+// clusters of 2 or 4 as many do not (one row of [4096, 12288]: 15.0 us, in clusters of 2 10.9).  The runtime, asked
+// once per device and size, counts one CTA an SM for a kernel that allocates TMEM; by shared memory, registers and TMEM two
+// fit, and two run.  0: the runtime gave an error.
+int cluster_capacity(int c) {
+  static std::atomic<int> known[64][9];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  if (dev < 64)
+    if (const int n = known[dev][c].load(std::memory_order_relaxed); n != 0) return n;
+  auto kernel = swap::linear_swap<false, 64>;
+  static unsigned long long configured = 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(c));
+  cfg.blockDim = dim3(swap::kThreads);
+  cfg.dynamicSmemBytes = swap::kSmemBytes;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(c);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int clusters = 0;
+  if (set_smem_once(kernel, static_cast<int>(swap::kSmemBytes), configured) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess || clusters < 1) {
+    cudaGetLastError();
+    return 0;
+  }
+  if (dev < 64) known[dev][c].store(2 * clusters * c, std::memory_order_relaxed);
+  return 2 * clusters * c;
+}
+
+struct SwapPlan {
+  int row_tiles, rows, parts;  // parts: of K, a cluster's CTAs
+  double us;
+};
+SwapPlan swap_plan(int64_t m, int64_t n, int k_blocks) {
+  SwapPlan s;
+  s.row_tiles = static_cast<int>((m + swap::kMostRows - 1) / swap::kMostRows);
+  s.rows = static_cast<int>(((m + s.row_tiles - 1) / s.row_tiles + 15) / 16 * 16);
+  const double tiles = static_cast<double>((n + swap::BN - 1) / swap::BN) * s.row_tiles;
+  s.parts = 1;
+  s.us = 0.0;
+  for (int c = 1; c <= 8 && c <= k_blocks; ++c) {
+    const int room = cluster_capacity(c);
+    if (room == 0) continue;
+    const double waves = std::ceil(tiles * c / room), block = c > 1 ? 0.3 + 0.012 * s.rows : 0.2 + 0.0065 * s.rows;
+    const double us = 3.5 + waves * ((c > 1 ? 4.0 : 2.5) + (k_blocks + c - 1) / c * block);
+    if (s.us == 0.0 || us < s.us) {
+      s.us = us;
+      s.parts = c;
+    }
+  }
+  return s;
+}
+double pair_us(int64_t m, int64_t n, int k_blocks, int sms) {
+  const double tiles = static_cast<double>((m + 2 * pair::BM - 1) / (2 * pair::BM)) * ((n + pair::BN - 1) / pair::BN);
+  return 6.5 + 0.6 * k_blocks * std::ceil(tiles / (sms / 2));
+}
+
 template <bool kF32Out, int kRows>
 cudaError_t launch_swap_as(const Product& p, int rows, int row_tiles) {
   using namespace swap;
@@ -714,19 +786,8 @@ cudaError_t launch_swap_as(const Product& p, int rows, int row_tiles) {
   if (!make_map(&ta, p.enc, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.a, p.m, p.k, rows) ||
       !make_map(&tw, p.enc, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.w, p.n, p.k, BN))
     return cudaErrorInvalidValue;
-  const int64_t n_tiles = (p.n + BN - 1) / BN, tiles = n_tiles * row_tiles;
-  // K's parts: as few blocks of K one after another as the 2 CTAs of every SM allow, a CTA's beginning and end counted
-  // as kEnds blocks.
-  constexpr int kEnds = 6;
-  int parts = 1;
-  int64_t best = 0;
-  for (int c = 1; c <= 8 && c <= p.k_blocks; ++c) {
-    const int64_t waves = (tiles * c + 2 * p.sms - 1) / (2 * p.sms), cost = waves * ((p.k_blocks + c - 1) / c + kEnds);
-    if (c == 1 || cost < best) {
-      best = cost;
-      parts = c;
-    }
-  }
+  const int64_t n_tiles = (p.n + BN - 1) / BN;
+  const int parts = swap_plan(p.m, p.n, p.k_blocks).parts;
   int stages = kRingBytes / (kWBytes + rows * kRowBytes);
   if (stages > kMostStages) stages = kMostStages;
   return launch_cluster(kernel, dim3(static_cast<unsigned>(n_tiles * parts), static_cast<unsigned>(row_tiles)),
@@ -736,8 +797,8 @@ cudaError_t launch_swap_as(const Product& p, int rows, int row_tiles) {
 
 template <bool kF32Out>
 cudaError_t launch_swap(const Product& p) {
-  const int row_tiles = static_cast<int>((p.m + swap::kMostRows - 1) / swap::kMostRows);
-  const int rows = static_cast<int>(((p.m + row_tiles - 1) / row_tiles + 15) / 16 * 16);
+  const SwapPlan plan = swap_plan(p.m, p.n, p.k_blocks);
+  const int rows = plan.rows, row_tiles = plan.row_tiles;
   return rows <= 16    ? launch_swap_as<kF32Out, 16>(p, rows, row_tiles)
          : rows <= 32  ? launch_swap_as<kF32Out, 32>(p, rows, row_tiles)
                        : launch_swap_as<kF32Out, 64>(p, rows, row_tiles);
@@ -763,6 +824,8 @@ extern "C" int sl_linear_block_fp8(const uint8_t* a, const float* a_scales, cons
   const Product p{a, w, a_scales, w_scales, bias, m, n, k, y, y_type == SL_F32, static_cast<int>((k + BK - 1) / BK),
                   device.sms, encoder(), device.err, static_cast<cudaStream_t>(stream)};
   if (p.enc == nullptr || p.err == nullptr || p.sms < 2) return SL_CUDA_ERROR;
-  if (m <= 3 * swap::kMostRows) return status_of(p.f32 ? launch_swap<true>(p) : launch_swap<false>(p));
+  // A tile of up to 64 rows is always the few-rows kernel's; the grid's second dimension bounds its tiles.
+  if (m <= swap::kMostRows || (m <= 1024 && swap_plan(m, n, p.k_blocks).us < pair_us(m, n, p.k_blocks, p.sms)))
+    return status_of(p.f32 ? launch_swap<true>(p) : launch_swap<false>(p));
   return status_of(launch_pair(p));
 }
