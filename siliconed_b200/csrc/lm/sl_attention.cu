@@ -4,14 +4,17 @@
 //
 // One pass over the cache with a running maximum and sum (the online softmax).  Bound by HBM: every key and value of
 // the contexts is read once and used for the heads / kv_heads query heads that share it, 2 to 4 operations a byte
-// and query head.
+// and query head.  Measured (B200, 32 query on 8 key-value heads of 128, calls after one another): 8 contexts of 65536 tokens
+// in bf16 6.4 TB/s (0.99 of a copy's rate), in e4m3 6.2; 33 ragged contexts of up to 4400 tokens 5.4; one context of
+// 131072 (4 key-value heads) 54 us, 5.0 TB/s, of 513 tokens 9 us, of 16 tokens 5 us.
 //
-// Work.  The contexts of all (sequence, key-value head) pairs are laid end to end in units of 64 tokens, and every
-// CTA takes an equal share of consecutive units, whatever the lengths are: a share may end one pair's context and
-// begin the next one's.  A context that lies in one share is finished there.  Where a context is cut between
-// CTAs each writes its part's maximum, sum and unnormalised output to the workspace; the last to arrive (a counter
-// that it sets back to zero) adds the parts in the order of the shares, so every call gives the same bits.  A CTA
-// leaves at most two parts (its first and its last context), so the workspace does not grow with the batch.
+// Work.  The contexts of all (sequence, key-value head) pairs are laid end to end in units (a step of every warp of a
+// CTA, plus one per context) and every CTA takes an equal share of consecutive units, whatever the lengths are: a share
+// may end one pair's context and begin the next one's.  A context that lies in one share is finished there.  Where a
+// context is cut between CTAs each writes its part's maximum, sum and unnormalised output to the workspace; the last to
+// arrive (a counter that it sets back to zero) adds the parts in the order of the shares, so every call gives the same
+// bits.  A CTA leaves at most two parts (its first and its last context), so the workspace does not grow with the batch.
+// (A queue that hands out the last quarter of the units in smaller pieces measured no faster.)
 //
 // Inside a CTA each warp takes steps of 32 tokens with a maximum, sum and output of its own, joined through shared
 // memory at the context's end.  Both products run on mma.sync m16n8k16 with the cache as the A operand:

@@ -85,7 +85,7 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile in
   unsigned long long since = 0;
   for (uint32_t i = 1;; ++i) {
     if (sc::mbar_try_wait(bar, parity)) return true;
-    if ((i & 255u) != 0) continue;
+    if ((i & 31u) != 0) continue;
     if (*abort) return false;
     const unsigned long long now = sc::global_ns();
     if (since == 0) since = now;

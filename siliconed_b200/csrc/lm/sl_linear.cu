@@ -12,13 +12,16 @@
 //   tiles.  Each CTA loads its own 128 rows of a and of w by TMA (128-byte swizzle).  The tile leaves through shared
 //   memory by TMA stores, which run under the next tile's blocks.  What bounds it is a block's round trip through its TMEM
 //   buffer: 4 MMAs (650 cycles beside the epilogue's work), their commit (350), the partial read by 16 warps (450) and the
-//   buffer's release to the MMA thread (400), some 1900 cycles for the two buffers that 256 columns leave.  [4096, 3840] x
-//   [3840, 10240]: 186 us, 1730 TFLOP/s; without the epilogue's arithmetic 134 us, the loads take less.  (Tiles of 256 x
+//   buffer's release to the MMA threads (400), some 1900 cycles for the two buffers that 256 columns leave.  [4096, 3840] x
+//   [3840, 10240]: 182 us, 1770 TFLOP/s; without the epilogue's arithmetic 134 us, the loads take less.  (Tiles of 256 x
 //   128 with four buffers: 198 us, their MMAs read shared memory half again as often.  fma.rn.f32x2 for the sums: 293 us,
 //   pairs of registers moved together.  One issuing thread: 212 us.)
 // - linear_swap: for few rows, bound by reading the weight.  The operands change places: 128 weight rows are the MMA's
 //   M and the rows of a, in tiles of up to 64, its N, so that no MMA row or TMEM column is padding; K is cut over the
-//   CTAs of a cluster, whose partials meet through distributed shared memory and are added in rank order.
+//   CTAs of a cluster, whose partials meet through distributed shared memory and are added in rank order.  The weight's
+//   tiles are prefetched to L2 while the kernel before this one ends.  One row of [4096, 12288]: 11.0 us, 4.6 TB/s (0.71
+//   of a copy's rate); 64 rows of it 17.8 us, 131 rows of [2560, 9728] 15.6 us (a block of 64 rows takes a CTA's four
+//   epilogue warps some 700 cycles, its begin and end 6000).
 //
 // Rows past m or n and values past k arrive as zeros.  Every wait is bounded; no load uses cluster multicast.
 #include <atomic>

@@ -6,7 +6,8 @@
 // Bound by HBM: every value of x and delta is read once, x_out and the codes are written once.  One CTA per row
 // keeps z in registers between the sum of squares and the quantization, eight consecutive values a thread and
 // step (16 bytes of bf16, 32 of fp32); 16 neighbouring lanes hold one block of 128, so a block's maximum takes
-// four shuffles.
+// four shuffles.  Measured (B200): [4608, 3840] fp32 + fp32 38 us, 6.1 TB/s (0.94 of a copy's rate); one row of 2560
+// 2.7 us in a chain of calls.
 #include "sl_common.cuh"
 
 namespace sl {
