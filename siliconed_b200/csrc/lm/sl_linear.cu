@@ -544,18 +544,37 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     const int col = quarter * 32 + lane;
     if (parts == 1) {
+      // Through shared memory (over the ring, as below), so that the rows leave 16 bytes a lane.  (Two bytes a lane straight
+      // from the registers: 3900 cycles for 48 rows.)
       const float add = bias_at(bias, n0 + col, n);
-      if (n0 + col < n) {
+      constexpr int kSize = kF32Out ? 4 : 2, kPer = 16 / kSize;       // bytes of a value, values of 16 bytes
 #pragma unroll
-        for (int j = 0; j < kRows; ++j)
-          if (j < rows && m0 + j < m) {
-            const float v = acc[j] + add;
-            const int64_t at = static_cast<int64_t>(m0 + j) * n + n0 + col;
-            if (kF32Out)
-              static_cast<float*>(y)[at] = v;
-            else
-              static_cast<__nv_bfloat16*>(y)[at] = __float2bfloat16_rn(v);
-          }
+      for (int j = 0; j < kRows; ++j)
+        if (j < rows) {
+          if (kF32Out)
+            reinterpret_cast<float*>(ring)[j * BN + col] = acc[j] + add;
+          else
+            reinterpret_cast<__nv_bfloat16*>(ring)[j * BN + col] = __float2bfloat16_rn(acc[j] + add);
+        }
+      sc::named_barrier_sync(1, kEpiThreads);
+      const int live = min(rows, m - m0);
+      const bool wide = n % kPer == 0;  // rows of y start on 16 bytes
+      for (int i = et; i < live * (BN / kPer); i += kEpiThreads) {
+        const int t = i / (BN / kPer), c = i % (BN / kPer) * kPer;
+        const uint8_t* from = ring + (t * BN + c) * kSize;
+        uint8_t* to = static_cast<uint8_t*>(y) + (static_cast<int64_t>(m0 + t) * n + n0 + c) * kSize;
+        if (wide && n0 + c < n) {
+          *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from);
+        } else if (!wide) {
+#pragma unroll
+          for (int e = 0; e < kPer; ++e)
+            if (n0 + c + e < n) {
+              if (kF32Out)
+                reinterpret_cast<float*>(to)[e] = reinterpret_cast<const float*>(from)[e];
+              else
+                reinterpret_cast<uint16_t*>(to)[e] = reinterpret_cast<const uint16_t*>(from)[e];
+            }
+        }
       }
     } else {
       // Over the ring: every copy has arrived and every MMA has read it, or the wait for the last partial gave up and
