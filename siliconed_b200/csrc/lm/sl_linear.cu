@@ -20,8 +20,9 @@
 //   M and the rows of a, in tiles of up to 64, its N, so that no MMA row or TMEM column is padding; K is cut over the
 //   CTAs of a cluster, whose partials meet through distributed shared memory and are added in rank order.  The weight's
 //   tiles are prefetched to L2 while the kernel before this one ends.  One row of [4096, 12288]: 11.0 us, 4.6 TB/s (0.71
-//   of a copy's rate); 64 rows of it 17.8 us, 131 rows of [2560, 9728] 15.6 us (a block of 64 rows takes a CTA's four
-//   epilogue warps some 700 cycles, its begin and end 6000).
+//   of a copy's rate); 64 rows of it 17.8 us, 131 rows of [2560, 9728] 14.9 us: a block of 64 rows keeps shared memory
+//   busy for some 640 cycles (its copies, the MMAs' operands, and the factors, which every thread reads 16 bytes at a time:
+//   without them 12.2 us); eight epilogue warps spill and are slower.
 //
 // Rows past m or n and values past k arrive as zeros.  Every wait is bounded; no load uses cluster multicast.
 #include <atomic>
@@ -595,7 +596,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int col = n0 + 2 * cp;
     const float b0 = bias_at(bias, col, n), b1 = bias_at(bias, col + 1, n);
     const bool both = n % 2 == 0 && col + 1 < n;
-    for (int t = lo + group; t < hi && m0 + t < m; t += kThreads / (BN / 2)) {
+    constexpr int kAdders = kThreads / (BN / 2);  // whole groups of threads
+    for (int t = lo + group; group < kAdders && t < hi && m0 + t < m; t += kAdders) {
       const float* mine = reinterpret_cast<const float*>(ring) + t * BN + 2 * cp;
       float2 sum = make_float2(0.0f, 0.0f);
       for (uint32_t q = 0; q < parts; ++q) {
