@@ -19,10 +19,11 @@
 // - linear_swap: for few rows, bound by reading the weight.  The operands change places: 128 weight rows are the MMA's
 //   M and the rows of a, in tiles of up to 64, its N, so that no MMA row or TMEM column is padding; K is cut over the
 //   CTAs of a cluster, whose partials meet through distributed shared memory and are added in rank order.  The weight's
-//   tiles are prefetched to L2 while the kernel before this one ends.  One row of [4096, 12288]: 11.0 us, 4.6 TB/s (0.71
-//   of a copy's rate); 64 rows of it 17.8 us, 131 rows of [2560, 9728] 14.9 us: a block of 64 rows keeps shared memory
-//   busy for some 640 cycles (its copies, the MMAs' operands, and the factors, which every thread reads 16 bytes at a time:
-//   without them 12.2 us); eight epilogue warps spill and are slower.
+//   first tiles are prefetched to L2 while the kernel before this one ends.  One row of [4096, 12288] (from HBM, calls after
+//   one another): 12.0 us, 4.2 TB/s (0.65 of a copy's rate); 64 rows of it 17.8 us, 131 rows of [2560, 9728] 14.0 us: a block of
+//   64 rows keeps shared memory busy for some 640 cycles (its copies, the MMAs' operands, and the factors, which every
+//   thread reads 16 bytes at a time: without them 2.7 us less); eight epilogue warps spill and are slower.  (Room for a third
+//   CTA an SM, so that the next call's begin early: 15.4 us for one row, the CTAs spread unevenly.)
 //
 // Rows past m or n and values past k arrive as zeros.  Every wait is bounded; no load uses cluster multicast.
 #include <atomic>
@@ -383,6 +384,9 @@ struct Control {
 };
 constexpr size_t kSmemBytes = kRingBytes + 1024;
 static_assert(kMostRows * BN * 4 <= kRingBytes, "a partial fits the ring");
+// Every wait's parity tells one phase from the next as long as nobody is two phases ahead: the MMAs of block g wait for
+// the epilogue to have read block g - kBuffers, so a stage must not come round sooner than a buffer.
+static_assert(kRingBytes / (kWBytes + kMostRows * kRowBytes) >= kBuffers && kMostStages >= kBuffers, "stages for the buffers");
 
 // kRows: the sums' registers (16, 32 or 64); `rows` <= kRows is the tile's count, a multiple of 16, and the rows of
 // a's TMA box.
@@ -422,10 +426,11 @@ __global__ void __launch_bounds__(kThreads, 2)
     sc::tmem_alloc(&s.tmem_base, kTmemCols);
     sc::tmem_relinquish();
   }
-  // The weight on its way to L2 while the kernel before this one ends: L2 holds what that kernel writes too, so nothing
-  // stale can come of it.
+  // The ring's first blocks of the weight on their way to L2 while the kernel before this one ends: L2 holds what that
+  // kernel writes too, so nothing stale can come of it.  (All of the CTA's blocks at once: 13.0 us instead of 11.9 for one row
+  // of [4096, 12288], 11.9 instead of 11.7 without any.)
   if (warp == kEpiWarp0 && lane == 0)
-    for (int kb = kb0; kb < kb1; ++kb)
+    for (int kb = kb0; kb < kb1 && kb < kb0 + stages; ++kb)
       asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(&tm_w)),
                    "r"(kb * BK), "r"(n0)
                    : "memory");
@@ -731,15 +736,14 @@ cudaError_t launch_pair(const Product& p) {
   return tma ? launch_pair_as<false, true>(p) : launch_pair_as<false, false>(p);
 }
 
-// Estimated microseconds (B200, fitted to [m, 2560] x [2560, 9728], [m, 4096] x [4096, 12288 or 4096] and [m, 9728] x
-// [9728, 2560], m 1 to 1024; most within 20 %).  The few-rows kernel: waves of two CTAs an SM, a beginning and an end
-// each, and blocks one after another, slower where a cluster shares K.  The many-rows kernel: a tile's blocks one after
-// another.
-// How many CTAs of the few-rows kernel run at once in clusters of `c` (its instances differ in nothing that matters to that).
-// A cluster lies in one group of SMs, so some sizes leave slots empty: 288 CTAs in clusters of 3 took a second wave, in
-// clusters of 2 or 4 as many do not (one row of [4096, 12288]: 15.0 us, in clusters of 2 10.9).  The runtime, asked
-// once per device and size, counts one CTA an SM for a kernel that allocates TMEM; by shared memory, registers and TMEM two
-// fit, and two run.  0: the runtime gave an error.
+// A kernel that never runs, with the few-rows kernel's threads and room: what the runtime says of it holds for that one, of
+// which it would count one CTA an SM because it allocates TMEM (of which two fit).
+__global__ void __launch_bounds__(swap::kThreads, 2) seat() {}
+
+// How many CTAs of the few-rows kernel run at once in clusters of `c`, two an SM.  A cluster lies in one group of SMs, so
+// most sizes leave slots empty: 148 SMs hold 296 CTAs in clusters of 2, 279 of 3, 284 of 4, 280, 270, 259 and 264 of 5 to 8,
+// and the first CTA past that starts a second wave (one row, k 5120 to 10240: 10.5 us up to 284 in clusters of 4, 14.8
+// from 288).  The runtime is asked once per device and size.  0: it gave an error.
 int cluster_capacity(int c) {
   static std::atomic<int> known[64][9];
   int dev = 0;
@@ -749,12 +753,12 @@ int cluster_capacity(int c) {
   }
   if (dev < 64)
     if (const int n = known[dev][c].load(std::memory_order_relaxed); n != 0) return n;
-  auto kernel = swap::linear_swap<false, 64>;
   static unsigned long long configured = 0;
+  constexpr size_t kRoom = swap::kSmemBytes + sizeof(swap::Control);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(c));
   cfg.blockDim = dim3(swap::kThreads);
-  cfg.dynamicSmemBytes = swap::kSmemBytes;
+  cfg.dynamicSmemBytes = kRoom;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = static_cast<unsigned>(c);
@@ -763,41 +767,51 @@ int cluster_capacity(int c) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   int clusters = 0;
-  if (set_smem_once(kernel, static_cast<int>(swap::kSmemBytes), configured) != cudaSuccess ||
-      cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess || clusters < 1) {
+  if (set_smem_once(seat, static_cast<int>(kRoom), configured) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&clusters, seat, &cfg) != cudaSuccess || clusters < 1) {
     cudaGetLastError();
     return 0;
   }
-  if (dev < 64) known[dev][c].store(2 * clusters * c, std::memory_order_relaxed);
-  return 2 * clusters * c;
+  if (dev < 64) known[dev][c].store(clusters * c, std::memory_order_relaxed);
+  return clusters * c;
 }
 
+// Estimated microseconds with the weight in HBM, fitted (B200) to [m, 4096] x [4096, 12288 or 4096], [m, 12288] x [12288, 4096],
+// [m, 2560] x [2560, 9728 or 2560], [m, 9728] x [9728, 2560] and [m, 512] x [512, 1000], m 1 to 1024 and 1 to 8 parts; most
+// within 10 %.  The few-rows kernel: a begin and an end, longer where a cluster adds (and then for every wave); a CTA's
+// blocks one after another, slower with more rows and more CTAs an SM, so that a last wave of few CTAs is shorter; and the
+// weight's bytes.  The parts this picks are the fastest or within 3 % of them.
 struct SwapPlan {
   int row_tiles, rows, parts;  // parts: of K, a cluster's CTAs
   double us;
 };
-SwapPlan swap_plan(int64_t m, int64_t n, int k_blocks) {
+SwapPlan swap_plan(int64_t m, int64_t n, int k_blocks, int sms) {
   SwapPlan s;
   s.row_tiles = static_cast<int>((m + swap::kMostRows - 1) / swap::kMostRows);
   s.rows = static_cast<int>(((m + s.row_tiles - 1) / s.row_tiles + 15) / 16 * 16);
-  const double tiles = static_cast<double>((n + swap::BN - 1) / swap::BN) * s.row_tiles;
+  const double n_tiles = static_cast<double>((n + swap::BN - 1) / swap::BN);
   s.parts = 1;
   s.us = 0.0;
   for (int c = 1; c <= 8 && c <= k_blocks; ++c) {
     const int room = cluster_capacity(c);
     if (room == 0) continue;
-    const double waves = std::ceil(tiles * c / room), block = c > 1 ? 0.3 + 0.012 * s.rows : 0.2 + 0.0065 * s.rows;
-    const double us = 3.5 + waves * ((c > 1 ? 4.0 : 2.5) + (k_blocks + c - 1) / c * block);
-    if (s.us == 0.0 || us < s.us) {
+    const double ctas = n_tiles * s.row_tiles * c, full = std::ceil(ctas / room) - 1.0, last = ctas - full * room;
+    const auto blocks = [&](double at_once) {
+      return (k_blocks + c - 1) / c * (0.1 + s.rows * ((c > 1 ? 0.0058 : 0.0047) + 0.0015 * at_once / sms));
+    };
+    const double us = (c > 1 ? 4.2 * (full + 1.0) : 2.9) + full * blocks(room) + blocks(last) + n_tiles * k_blocks * 1.27e-3;
+    if (s.us == 0.0 || us <= s.us) {
       s.us = us;
       s.parts = c;
     }
   }
   return s;
 }
+// The many-rows kernel: a tile's blocks one after another, and the weight's bytes.
 double pair_us(int64_t m, int64_t n, int k_blocks, int sms) {
-  const double tiles = static_cast<double>((m + 2 * pair::BM - 1) / (2 * pair::BM)) * ((n + pair::BN - 1) / pair::BN);
-  return 6.5 + 0.6 * k_blocks * std::ceil(tiles / (sms / 2));
+  const double n_tiles = static_cast<double>((n + pair::BN - 1) / pair::BN);
+  const double waves = std::ceil(static_cast<double>((m + 2 * pair::BM - 1) / (2 * pair::BM)) * n_tiles / (sms / 2));
+  return 6.3 + k_blocks * (0.63 * waves - 0.1) + n_tiles * k_blocks * 1.6e-3;
 }
 
 template <bool kF32Out, int kRows>
@@ -811,7 +825,7 @@ cudaError_t launch_swap_as(const Product& p, int rows, int row_tiles) {
       !make_map(&tw, p.enc, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.w, p.n, p.k, BN))
     return cudaErrorInvalidValue;
   const int64_t n_tiles = (p.n + BN - 1) / BN;
-  const int parts = swap_plan(p.m, p.n, p.k_blocks).parts;
+  const int parts = swap_plan(p.m, p.n, p.k_blocks, p.sms).parts;
   int stages = kRingBytes / (kWBytes + rows * kRowBytes);
   if (stages > kMostStages) stages = kMostStages;
   return launch_cluster(kernel, dim3(static_cast<unsigned>(n_tiles * parts), static_cast<unsigned>(row_tiles)),
@@ -821,7 +835,7 @@ cudaError_t launch_swap_as(const Product& p, int rows, int row_tiles) {
 
 template <bool kF32Out>
 cudaError_t launch_swap(const Product& p) {
-  const SwapPlan plan = swap_plan(p.m, p.n, p.k_blocks);
+  const SwapPlan plan = swap_plan(p.m, p.n, p.k_blocks, p.sms);
   const int rows = plan.rows, row_tiles = plan.row_tiles;
   return rows <= 16    ? launch_swap_as<kF32Out, 16>(p, rows, row_tiles)
          : rows <= 32  ? launch_swap_as<kF32Out, 32>(p, rows, row_tiles)
@@ -848,8 +862,11 @@ extern "C" int sl_linear_block_fp8(const uint8_t* a, const float* a_scales, cons
   const Product p{a, w, a_scales, w_scales, bias, m, n, k, y, y_type == SL_F32, static_cast<int>((k + BK - 1) / BK),
                   device.sms, encoder(), device.err, static_cast<cudaStream_t>(stream)};
   if (p.enc == nullptr || p.err == nullptr || p.sms < 2) return SL_CUDA_ERROR;
-  // A tile of up to 64 rows is always the few-rows kernel's; the grid's second dimension bounds its tiles.
-  if (m <= swap::kMostRows || (m <= 1024 && swap_plan(m, n, p.k_blocks).us < pair_us(m, n, p.k_blocks, p.sms)))
+  // Up to 64 rows are always the few-rows kernel's; its row tiles are the grid's second dimension.  (Both measured, us, few-rows
+  // and many-rows kernel: [m, 2560] x [2560, 9728] 15.5 and 18.3 at 192 rows, 25.3 and 18.5 at 256, 29.1 and 31.3 at 384;
+  // [m, 4096] x [4096, 4096] 22.1 and 23.7 at 512, 43.5 and 24.3 at 640.)
+  if (m <= swap::kMostRows || (m <= int64_t{65535} * swap::kMostRows &&
+                               swap_plan(m, n, p.k_blocks, p.sms).us < pair_us(m, n, p.k_blocks, p.sms)))
     return status_of(p.f32 ? launch_swap<true>(p) : launch_swap<false>(p));
   return status_of(launch_pair(p));
 }
