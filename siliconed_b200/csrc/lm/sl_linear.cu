@@ -268,17 +268,44 @@ __global__ void __launch_bounds__(kThreads, 1)
             bulk_commit();
           }
         }
-      } else if (row < m) {
-        const int64_t at = static_cast<int64_t>(row) * n + col0;
+      } else {
+        // Rows that do not start on 16 bytes: through shared memory all the same, so that a warp's stores are of neighbours.
+        // (Every lane along its own row: 178 us for [2000, 9728] x [9728, 2567], this way 98; 94 for 2560 columns.)
+        constexpr int kPassCols = kF32Out ? 64 : 128, kPer = kF32Out ? 4 : 8;  // 256 bytes of a row; values of 16 bytes
+        uint8_t* out = &s.out[ew][0][0];
+        const int rows = min(32, m - row0);
 #pragma unroll
-        for (int j = 0; j < BNH; ++j)
-          if (col0 + j < n) {
-            const float v = acc[j] + bias_at(bias, col0 + j, n);
-            if (kF32Out)
-              static_cast<float*>(y)[at + j] = v;
-            else
-              static_cast<__nv_bfloat16*>(y)[at + j] = __float2bfloat16_rn(v);
+        for (int b = 0; b < BNH / kPassCols; ++b) {
+          const int col = col0 + b * kPassCols;
+          __syncwarp();  // the pass before has been read
+#pragma unroll
+          for (int q = 0; q < 16; ++q) {
+            float x[8];
+#pragma unroll
+            for (int t = 0; t < kPer; ++t) x[t] = acc[b * kPassCols + q * kPer + t] + bias_at(bias, col + q * kPer + t, n);
+            const uint4 v = kF32Out ? make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]))
+                                    : pack8(x);
+            *reinterpret_cast<uint4*>(out + lane * 256 + ((q & 8 | ((q & 7) ^ (lane & 7))) << 4)) = v;
           }
+          __syncwarp();
+          const auto leave = [&](auto unit) {
+            using T = decltype(unit);
+            constexpr int kUnits = 256 / sizeof(T), kChunk = 16 / sizeof(T), kValues = kF32Out ? 1 : sizeof(T) / 2;
+            for (int t = 0; t < rows; ++t) {
+              T* to = reinterpret_cast<T*>(static_cast<uint8_t*>(y) + (static_cast<int64_t>(row0 + t) * n + col) * (kF32Out ? 4 : 2));
+#pragma unroll
+              for (int u = lane; u < kUnits; u += 32) {
+                const int chunk = u / kChunk;
+                if (col + u * kValues < n)
+                  to[u] = reinterpret_cast<const T*>(out + t * 256 + ((chunk & 8 | ((chunk & 7) ^ (t & 7))) << 4))[u % kChunk];
+              }
+            }
+          };
+          if (kF32Out || n % 2 == 0)
+            leave(uint32_t{});
+          else
+            leave(uint16_t{});
+        }
       }
     }
     if (kTmaOut && lane == 0) bulk_wait_all();
@@ -383,6 +410,7 @@ struct Control {
   alignas(16) float factors[2][kGroup][kMostRows];  // sa * sw of a group of blocks, by the group's parity
 };
 constexpr size_t kSmemBytes = kRingBytes + 1024;
+static_assert(kEpiThreads == BN, "a thread per column");
 static_assert(kMostRows * BN * 4 <= kRingBytes, "a partial fits the ring");
 // Every wait's parity tells one phase from the next as long as nobody is two phases ahead: the MMAs of block g wait for
 // the epilogue to have read block g - kBuffers, so a stage must not come round sooner than a buffer.
@@ -550,10 +578,10 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     const int col = quarter * 32 + lane;
     if (parts == 1) {
-      // Through shared memory (over the ring, as below), so that the rows leave 16 bytes a lane.  (Two bytes a lane straight
+      // Through shared memory (over the ring, as below), so that a warp's stores are of neighbours.  (Two bytes a lane straight
       // from the registers: 3900 cycles for 48 rows.)
       const float add = bias_at(bias, n0 + col, n);
-      constexpr int kSize = kF32Out ? 4 : 2, kPer = 16 / kSize;       // bytes of a value, values of 16 bytes
+      constexpr int kSize = kF32Out ? 4 : 2, kPer = 16 / kSize;  // bytes of a value, values of 16 bytes
 #pragma unroll
       for (int j = 0; j < kRows; ++j)
         if (j < rows) {
@@ -565,21 +593,21 @@ __global__ void __launch_bounds__(kThreads, 2)
       sc::named_barrier_sync(1, kEpiThreads);
       const int live = min(rows, m - m0);
       const bool wide = n % kPer == 0;  // rows of y start on 16 bytes
-      for (int i = et; i < live * (BN / kPer); i += kEpiThreads) {
-        const int t = i / (BN / kPer), c = i % (BN / kPer) * kPer;
-        const uint8_t* from = ring + (t * BN + c) * kSize;
-        uint8_t* to = static_cast<uint8_t*>(y) + (static_cast<int64_t>(m0 + t) * n + n0 + c) * kSize;
-        if (wide && n0 + c < n) {
-          *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from);
-        } else if (!wide) {
-#pragma unroll
-          for (int e = 0; e < kPer; ++e)
-            if (n0 + c + e < n) {
-              if (kF32Out)
-                reinterpret_cast<float*>(to)[e] = reinterpret_cast<const float*>(from)[e];
-              else
-                reinterpret_cast<uint16_t*>(to)[e] = reinterpret_cast<const uint16_t*>(from)[e];
-            }
+      if (wide) {
+        for (int i = et; i < live * (BN / kPer); i += kEpiThreads) {
+          const int t = i / (BN / kPer), c = i % (BN / kPer) * kPer;
+          if (n0 + c < n)
+            *reinterpret_cast<uint4*>(static_cast<uint8_t*>(y) + (static_cast<int64_t>(m0 + t) * n + n0 + c) * kSize) =
+                *reinterpret_cast<const uint4*>(ring + (t * BN + c) * kSize);
+        }
+      } else if (n0 + et < n) {  // a value a lane, a row a step
+#pragma unroll 1
+        for (int t = 0; t < live; ++t) {
+          const int64_t at = static_cast<int64_t>(m0 + t) * n + n0 + et;
+          if (kF32Out)
+            static_cast<float*>(y)[at] = reinterpret_cast<const float*>(ring)[t * BN + et];
+          else
+            static_cast<uint16_t*>(y)[at] = reinterpret_cast<const uint16_t*>(ring)[t * BN + et];
         }
       }
     } else {

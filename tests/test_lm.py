@@ -581,6 +581,25 @@ def test_linear_block_fp8(m, n, k):
 
 @gpu
 @needs_cuda
+@pytest.mark.parametrize("m,n", [(150, 9727), (700, 5001), (700, 5002), (705, 5004), (700, 5008), (2001, 2567)])
+def test_linear_rows_that_start_on_any_value(m, n):
+    """Outputs whose rows start on 2, 4, 8 and 16 bytes, from both kernels, and nothing written past them."""
+    g = gen(n)
+    k = 1040
+    _, codes, scales = lm_abi.rms_norm_quantize(torch.randn(m, k, generator=g, device="cuda"), norm=False)
+    w, ws = block_weight(g, n, k)
+    bias = torch.randn(n, generator=g, device="cuda").to(BF)
+    for dtype in (BF, torch.float32):
+        room = torch.full((m * n + 4096,), -7.0, dtype=dtype, device="cuda")
+        y = room[:m * n].view(m, n)
+        lm_abi.linear_block_fp8(codes, scales, w, ws, bias, y)
+        check_product(codes, scales, w, ws, bias, y)
+        assert bool((room[m * n:] == -7.0).all())
+    clean()
+
+
+@gpu
+@needs_cuda
 @pytest.mark.parametrize("m", [3, 40, 500])
 def test_linear_keeps_scales_apart_and_nan_in_its_row(m):
     """Scales of very different sizes (a block's partial product must not be rounded against another's), a NaN block."""
