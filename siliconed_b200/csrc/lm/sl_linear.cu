@@ -15,7 +15,10 @@
 //   buffer's release to the MMA threads (400), some 1900 cycles for the two buffers that 256 columns leave.  [4096, 3840] x
 //   [3840, 10240]: 182 us, 1770 TFLOP/s; without the epilogue's arithmetic 134 us, the loads take less.  (Tiles of 256 x
 //   128 with four buffers: 198 us, their MMAs read shared memory half again as often.  fma.rn.f32x2 for the sums: 293 us,
-//   pairs of registers moved together.  One issuing thread: 212 us.)
+//   pairs of registers moved together.  One issuing thread: 212 us.  The two halves of the columns issued by a thread
+//   each, two buffers each: 5 % slower, a is read twice.  16 epilogue warps of 64 columns: 258 us, spills.)  Where the
+//   tiles leave pairs idle, a cluster of up to 4 pairs shares a tile's K and adds its parts as below: [512, 9728] x [9728,
+//   2560] 24.7 us, 46.3 without.
 // - linear_swap: for few rows, bound by reading the weight.  The operands change places: 128 weight rows are the MMA's
 //   M and the rows of a, in tiles of up to 64, its N, so that no MMA row or TMEM column is padding; K is cut over the
 //   CTAs of a cluster, whose partials meet through distributed shared memory and are added in rank order.  The weight's
@@ -120,6 +123,8 @@ constexpr int kEpiRegisters = 232, kOtherRegisters = 40;
 constexpr int kLaunchRegisters = (kOtherRegisters + 2 * kEpiRegisters + 2) / 3;
 constexpr uint32_t kTmemCols = 512;       // two partial products of 256 columns
 constexpr int kBoxBytes = 32 * 128;       // 32 rows of 128 bytes of y: a TMA store
+constexpr int kPartRow = BN * 4;          // a row of a part's sums
+constexpr int kMostParts = 4;             // pairs of a cluster
 
 struct __align__(1024) Smem {
   uint8_t a[kStages][kTileBytes];
@@ -134,6 +139,7 @@ struct __align__(1024) Smem {
 };
 constexpr size_t kSmemBytes = sizeof(Smem) + 1024;
 static_assert(kSmemBytes <= 227 * 1024, "shared memory per CTA");
+static_assert(BM * kPartRow <= 2 * kStages * kTileBytes, "a part's sums fit the stages");
 
 // kTmaOut: y's rows start on 16 bytes, so that whole boxes leave by TMA.
 template <bool kF32Out, bool kTmaOut>
@@ -141,13 +147,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     linear_pair(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_w,
                 const __grid_constant__ CUtensorMap tm_y, const float* __restrict__ a_scales,
                 const float* __restrict__ w_scales, const uint16_t* __restrict__ bias, void* __restrict__ y, int m, int n,
-                int k_blocks, int m_tiles, int n_tiles, int* err) {
+                int k_blocks, int m_tiles, int n_tiles, int parts, int* err) {
   extern __shared__ uint8_t smem_raw[];
   Smem& s = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = sc::cluster_ctarank();
+  const uint32_t cluster_rank = sc::cluster_ctarank(), rank = cluster_rank & 1u, lead = cluster_rank & ~1u;
   const bool leader = rank == 0;
-  const int first = blockIdx.x >> 1, pairs = gridDim.x >> 1, tiles = m_tiles * n_tiles;
+  // `parts` pairs, a cluster, share a tile's K; above one part every cluster has one tile.
+  const int part = static_cast<int>(cluster_rank >> 1);
+  const int first = static_cast<int>(blockIdx.x) / (2 * parts), pairs = static_cast<int>(gridDim.x) / (2 * parts), tiles = m_tiles * n_tiles;
+  const int kb0 = part * k_blocks / parts, kb1 = (part + 1) * k_blocks / parts;
   volatile int* abort = &s.abort;
   sc::pdl_launch_dependents();
   if (threadIdx.x == 0) {
@@ -197,12 +206,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int j = 0; j < BNH; ++j) acc[j] = 0.0f;
       // The scales are asked for two blocks ahead, into registers of their own for even and odd blocks: handed from one
       // to the next they would have to arrive first (one block then took 2000 cycles instead of 750).
-      float a_even = sa[0], w_even = sw[0], a_odd = sa[min(1, k_blocks - 1)], w_odd = sw[min(1, k_blocks - 1)];
+      const int second = min(kb0 + 1, kb1 - 1);
+      float a_even = sa[kb0], w_even = sw[kb0], a_odd = sa[second], w_odd = sw[second];
       const auto add_block = [&](int kb, float& a_scale, float& w_scale) {
         if (!(ok = wait_warp(&s.done[stage], phase, abort, err, kSiteLinearSum))) return;
         sc::tc_fence_after();
         const float f = a_scale * w_scale;
-        const int next = min(kb + 2, k_blocks - 1);
+        const int next = min(kb + 2, kb1 - 1);
         a_scale = sa[next];
         w_scale = sw[next];
         uint32_t r[3][32];
@@ -223,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // All of the partial is in registers: its buffer is free.
         sc::tc_fence_before();
         __syncwarp();
-        if (lane == 0) sc::mbar_arrive_cluster(sc::peer_addr(&s.part_empty[buf], 0));
+        if (lane == 0) sc::mbar_arrive_cluster(sc::peer_addr(&s.part_empty[buf], lead));
         add(1, r[1]);
         add(2, r[2]);
         add(3, r[0]);
@@ -233,12 +243,20 @@ __global__ void __launch_bounds__(kThreads, 1)
           phase ^= 1u;
         }
       };
-      for (int kb = 0; kb < k_blocks && ok; kb += 2) {
+      for (int kb = kb0; kb < kb1 && ok; kb += 2) {
         add_block(kb, a_even, w_even);
-        if (kb + 1 < k_blocks && ok) add_block(kb + 1, a_odd, w_odd);
+        if (kb + 1 < kb1 && ok) add_block(kb + 1, a_odd, w_odd);
       }
       if (!ok) break;
-      if (kTmaOut) {
+      if (parts > 1) {
+        // The sums over the stages, which nothing reads or writes any more: a row of 256 floats a thread and its neighbour
+        // half, 16-byte chunks exchanged so that 8 lanes' writes meet different banks.
+        uint8_t* mine = s.a[0] + (quarter * 32 + lane) * kPartRow;
+#pragma unroll
+        for (int q = 0; q < BNH / 4; ++q)
+          *reinterpret_cast<float4*>(mine + ((half * (BNH / 4) + (q ^ (lane & 7))) << 4)) =
+              make_float4(acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]);
+      } else if (kTmaOut) {
         constexpr int kBoxCols = kF32Out ? 32 : 64;  // 128 bytes
         uint8_t* out = &s.out[ew][0][0];
 #pragma unroll
@@ -309,6 +327,52 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     if (kTmaOut && lane == 0) bulk_wait_all();
+    if (parts > 1) {
+      // Every part's pair adds a share of the rows, in the parts' order: the same sums whichever adds them.
+      sc::cluster_barrier();
+      int mt, nt;
+      sc::tile_coords(first, m_tiles, n_tiles, mt, nt);
+      const int row0 = (mt * 2 + static_cast<int>(rank)) * BM;
+      const int lo = part * BM / parts, hi = (part + 1) * BM / parts;
+      for (int t = lo + ew; t < hi && row0 + t < m; t += kEpiWarps)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int u = h * 32 + lane, col = nt * BN + 4 * u;
+          const uint8_t* from = s.a[0] + t * kPartRow + (((u & ~7) | ((u & 7) ^ (t & 7))) << 4);
+          float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          for (int q = 0; q < parts; ++q) {
+            float4 v;
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                         : "r"(sc::peer_addr(from, 2 * q + rank))
+                         : "memory");
+            sum.x += v.x;
+            sum.y += v.y;
+            sum.z += v.z;
+            sum.w += v.w;
+          }
+          const float out[4] = {sum.x + bias_at(bias, col, n), sum.y + bias_at(bias, col + 1, n), sum.z + bias_at(bias, col + 2, n),
+                                sum.w + bias_at(bias, col + 3, n)};
+          const int64_t at = static_cast<int64_t>(row0 + t) * n + col;
+          if (kTmaOut) {  // n a multiple of 4 at least
+            if (col < n) {
+              if (kF32Out)
+                *reinterpret_cast<float4*>(static_cast<float*>(y) + at) = make_float4(out[0], out[1], out[2], out[3]);
+              else
+                *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(y) + at) = make_uint2(pack_bf16x2(out[0], out[1]), pack_bf16x2(out[2], out[3]));
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (col + e < n) {
+                if (kF32Out)
+                  static_cast<float*>(y)[at + e] = out[e];
+                else
+                  static_cast<__nv_bfloat16*>(y)[at + e] = __float2bfloat16_rn(out[e]);
+              }
+          }
+        }
+    }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
     if (warp == 0) {
@@ -321,13 +385,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           int mt, nt;
           sc::tile_coords(tile, m_tiles, n_tiles, mt, nt);
           const int row0 = (mt * 2 + static_cast<int>(rank)) * BM, col0 = nt * BN + static_cast<int>(rank) * BNH;
-          for (int kb = 0; kb < k_blocks; ++kb) {
+          for (int kb = kb0; kb < kb1; ++kb) {
             if (!wait(&s.done[stage], phase ^ 1u, abort, err, kSiteLinearLoad)) {
               ok = false;
               break;
             }
             if (leader) sc::mbar_arrive_expect_tx(&s.full[stage], 4 * kTileBytes);
-            const uint32_t bar = sc::peer_addr(&s.full[stage], 0);
+            const uint32_t bar = sc::peer_addr(&s.full[stage], lead);
             sc::tma_load_2d_pair(s.a[stage], &tm_a, bar, kb * BK, row0);
             sc::tma_load_2d_pair(s.w[stage], &tm_w, bar, kb * BK, col0);
             issued |= 1u << stage;
@@ -348,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (leader && lane == 0) {
         constexpr uint32_t idesc = idesc_e4m3(2 * BM, BN);
         const int buf = warp - 1;
-        const int blocks = (tiles - first + pairs - 1) / pairs * k_blocks;  // of this pair's tiles
+        const int blocks = (tiles - first + pairs - 1) / pairs * (kb1 - kb0);  // of this pair's tiles
         int stage = buf;
         uint32_t phase = 0, buf_phase = 0;
         for (int g = buf; g < blocks; g += 2) {
@@ -361,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int kk = 0; kk < BK / 32; ++kk)
             mma_e4m3<true>(tmem + static_cast<uint32_t>(buf * BN), sc::umma_desc_sw128(a0 + kk * 32),
                            sc::umma_desc_sw128(b0 + kk * 32), idesc, kk != 0 ? 1u : 0u);
-          sc::tc_commit_pair_both(&s.done[stage], 0x3);
+          sc::tc_commit_pair_both(&s.done[stage], static_cast<uint16_t>(0x3u << lead));
           buf_phase ^= 1u;
           stage += 2;
           if (stage >= kStages) {
@@ -369,12 +433,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             phase ^= 1u;
           }
         }
-        sc::tc_commit_pair(sc::peer_addr(&s.drain[buf], 0));
+        sc::tc_commit_pair(sc::peer_addr(&s.drain[buf], lead));
         sc::mbar_wait_drain(&s.drain[buf], 0);
       }
     }
+    __syncwarp();
+    if (parts > 1) sc::cluster_barrier();
   }
-  // Neither CTA leaves while the pair's MMAs, TMEM or barriers may still reach its memory.
+  // No CTA leaves while the pair's MMAs, TMEM or barriers or the cluster's sums may still reach its memory.
   __syncwarp();
   sc::tc_fence_before();
   sc::cluster_barrier();
@@ -734,44 +800,16 @@ cudaError_t launch_cluster(void (*kernel)(Params...), dim3 grid, int threads, si
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
 }
 
-template <bool kF32Out, bool kTmaOut>
-cudaError_t launch_pair_as(const Product& p) {
-  using namespace pair;
-  auto kernel = linear_pair<kF32Out, kTmaOut>;
-  static unsigned long long configured = 0;
-  if (const cudaError_t e = set_smem_once(kernel, static_cast<int>(kSmemBytes), configured); e != cudaSuccess) return e;
-  static const int registers = [kernel] {
-    cudaFuncAttributes attr;
-    return cudaFuncGetAttributes(&attr, kernel) == cudaSuccess ? attr.numRegs : 0;
-  }();
-  if (registers < kLaunchRegisters) return cudaErrorLaunchOutOfResources;
-  CUtensorMap ta, tw, ty = {};
-  if (!make_map(&ta, p.enc, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.a, p.m, p.k, BM) ||
-      !make_map(&tw, p.enc, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.w, p.n, p.k, BNH) ||
-      (kTmaOut && !make_map(&ty, p.enc, kF32Out ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-                            kF32Out ? 4 : 2, p.y, p.m, p.n, 32)))
-    return cudaErrorInvalidValue;
-  const int m_tiles = static_cast<int>((p.m + 2 * BM - 1) / (2 * BM)), n_tiles = static_cast<int>((p.n + BN - 1) / BN);
-  const int64_t tiles = static_cast<int64_t>(m_tiles) * n_tiles;
-  const int pairs = static_cast<int>(tiles < p.sms / 2 ? tiles : p.sms / 2);
-  return launch_cluster(kernel, dim3(static_cast<unsigned>(2 * pairs)), kThreads, kSmemBytes, 2, p.stream, ta, tw, ty, p.a_scales,
-                        p.w_scales, p.bias, p.y, static_cast<int>(p.m), static_cast<int>(p.n), p.k_blocks, m_tiles, n_tiles, p.err);
-}
+// Kernels that never run, with the two kernels' threads and room: what the runtime says of them holds for those, of which it
+// would count one CTA an SM because they allocate TMEM (of the few-rows kernel two fit).
+__global__ void __launch_bounds__(swap::kThreads, 2) seat_swap() {}
+__global__ void __launch_bounds__(pair::kThreads, 1) seat_pair() {}
 
-cudaError_t launch_pair(const Product& p) {
-  const bool tma = p.n % (p.f32 ? 4 : 8) == 0;
-  if (p.f32) return tma ? launch_pair_as<true, true>(p) : launch_pair_as<true, false>(p);
-  return tma ? launch_pair_as<false, true>(p) : launch_pair_as<false, false>(p);
-}
-
-// A kernel that never runs, with the few-rows kernel's threads and room: what the runtime says of it holds for that one, of
-// which it would count one CTA an SM because it allocates TMEM (of which two fit).
-__global__ void __launch_bounds__(swap::kThreads, 2) seat() {}
-
-// How many CTAs of the few-rows kernel run at once in clusters of `c`, two an SM.  A cluster lies in one group of SMs, so
-// most sizes leave slots empty: 148 SMs hold 296 CTAs in clusters of 2, 279 of 3, 284 of 4, 280, 270, 259 and 264 of 5 to 8,
-// and the first CTA past that starts a second wave (one row, k 5120 to 10240: 10.5 us up to 284 in clusters of 4, 14.8
-// from 288).  The runtime is asked once per device and size.  0: it gave an error.
+// How many CTAs run at once in clusters of `c`.  A cluster lies in one group of SMs, so most sizes leave slots empty: for the
+// few-rows kernel, two CTAs an SM, 148 SMs hold 296 CTAs in clusters of 2, 279 of 3, 284 of 4, 280, 270, 259 and 264 of 5 to
+// 8, and the first CTA past that starts a second wave (one row, k 5120 to 10240: 10.5 us up to 284 in clusters of 4,
+// 14.8 from 288).  The runtime is asked once per device and size.  0: it gave an error.
+template <bool kPair>
 int cluster_capacity(int c) {
   static std::atomic<int> known[64][9];
   int dev = 0;
@@ -782,10 +820,11 @@ int cluster_capacity(int c) {
   if (dev < 64)
     if (const int n = known[dev][c].load(std::memory_order_relaxed); n != 0) return n;
   static unsigned long long configured = 0;
-  constexpr size_t kRoom = swap::kSmemBytes + sizeof(swap::Control);
+  constexpr size_t kRoom = kPair ? pair::kSmemBytes : swap::kSmemBytes + sizeof(swap::Control);
+  const auto seat = kPair ? seat_pair : seat_swap;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(c));
-  cfg.blockDim = dim3(swap::kThreads);
+  cfg.blockDim = dim3(kPair ? pair::kThreads : swap::kThreads);
   cfg.dynamicSmemBytes = kRoom;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -821,7 +860,7 @@ SwapPlan swap_plan(int64_t m, int64_t n, int k_blocks, int sms) {
   s.parts = 1;
   s.us = 0.0;
   for (int c = 1; c <= 8 && c <= k_blocks; ++c) {
-    const int room = cluster_capacity(c);
+    const int room = cluster_capacity<false>(c);
     if (room == 0) continue;
     const double ctas = n_tiles * s.row_tiles * c, full = std::ceil(ctas / room) - 1.0, last = ctas - full * room;
     const auto blocks = [&](double at_once) {
@@ -835,11 +874,55 @@ SwapPlan swap_plan(int64_t m, int64_t n, int k_blocks, int sms) {
   }
   return s;
 }
-// The many-rows kernel: a tile's blocks one after another, and the weight's bytes.
-double pair_us(int64_t m, int64_t n, int k_blocks, int sms) {
+// The many-rows kernel: a tile's blocks one after another, and the weight's bytes.  Where the tiles leave pairs idle, a cluster
+// of pairs shares each tile's K.
+struct PairPlan {
+  int parts;
+  double us;
+};
+PairPlan pair_plan(int64_t m, int64_t n, int k_blocks, int sms) {
   const double n_tiles = static_cast<double>((n + pair::BN - 1) / pair::BN);
-  const double waves = std::ceil(static_cast<double>((m + 2 * pair::BM - 1) / (2 * pair::BM)) * n_tiles / (sms / 2));
-  return 6.3 + k_blocks * (0.63 * waves - 0.1) + n_tiles * k_blocks * 1.6e-3;
+  const double tiles = static_cast<double>((m + 2 * pair::BM - 1) / (2 * pair::BM)) * n_tiles, waves = std::ceil(tiles / (sms / 2));
+  const double bytes = n_tiles * k_blocks * 1.6e-3;
+  PairPlan plan = {1, 6.3 + k_blocks * (0.63 * waves - 0.1) + bytes};
+  for (int c = 2; c <= pair::kMostParts && c <= k_blocks && tiles * c <= sms / 2; ++c) {
+    if (tiles * 2 * c > cluster_capacity<true>(2 * c)) continue;
+    const double us = 10.0 + (k_blocks + c - 1) / c * 0.53 + bytes;
+    if (us < plan.us) plan = {c, us};
+  }
+  return plan;
+}
+
+template <bool kF32Out, bool kTmaOut>
+cudaError_t launch_pair_as(const Product& p) {
+  using namespace pair;
+  auto kernel = linear_pair<kF32Out, kTmaOut>;
+  static unsigned long long configured = 0;
+  if (const cudaError_t e = set_smem_once(kernel, static_cast<int>(kSmemBytes), configured); e != cudaSuccess) return e;
+  static const int registers = [kernel] {
+    cudaFuncAttributes attr;
+    return cudaFuncGetAttributes(&attr, kernel) == cudaSuccess ? attr.numRegs : 0;
+  }();
+  if (registers < kLaunchRegisters) return cudaErrorLaunchOutOfResources;
+  CUtensorMap ta, tw, ty = {};
+  if (!make_map(&ta, p.enc, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.a, p.m, p.k, BM) ||
+      !make_map(&tw, p.enc, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.w, p.n, p.k, BNH) ||
+      (kTmaOut && !make_map(&ty, p.enc, kF32Out ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                            kF32Out ? 4 : 2, p.y, p.m, p.n, 32)))
+    return cudaErrorInvalidValue;
+  const int m_tiles = static_cast<int>((p.m + 2 * BM - 1) / (2 * BM)), n_tiles = static_cast<int>((p.n + BN - 1) / BN);
+  const int64_t tiles = static_cast<int64_t>(m_tiles) * n_tiles;
+  const int parts = pair_plan(p.m, p.n, p.k_blocks, p.sms).parts;
+  const int clusters = static_cast<int>(parts > 1 || tiles < p.sms / 2 ? tiles : p.sms / 2);
+  return launch_cluster(kernel, dim3(static_cast<unsigned>(2 * parts * clusters)), kThreads, kSmemBytes, 2 * parts, p.stream, ta, tw,
+                        ty, p.a_scales, p.w_scales, p.bias, p.y, static_cast<int>(p.m), static_cast<int>(p.n), p.k_blocks, m_tiles,
+                        n_tiles, parts, p.err);
+}
+
+cudaError_t launch_pair(const Product& p) {
+  const bool tma = p.n % (p.f32 ? 4 : 8) == 0;
+  if (p.f32) return tma ? launch_pair_as<true, true>(p) : launch_pair_as<true, false>(p);
+  return tma ? launch_pair_as<false, true>(p) : launch_pair_as<false, false>(p);
 }
 
 template <bool kF32Out, int kRows>
@@ -894,7 +977,7 @@ extern "C" int sl_linear_block_fp8(const uint8_t* a, const float* a_scales, cons
   // and many-rows kernel: [m, 2560] x [2560, 9728] 15.5 and 18.3 at 192 rows, 25.3 and 18.5 at 256, 29.1 and 31.3 at 384;
   // [m, 4096] x [4096, 4096] 22.1 and 23.7 at 512, 43.5 and 24.3 at 640.)
   if (m <= swap::kMostRows || (m <= int64_t{65535} * swap::kMostRows &&
-                               swap_plan(m, n, p.k_blocks, p.sms).us < pair_us(m, n, p.k_blocks, p.sms)))
+                               swap_plan(m, n, p.k_blocks, p.sms).us < pair_plan(m, n, p.k_blocks, p.sms).us))
     return status_of(p.f32 ? launch_swap<true>(p) : launch_swap<false>(p));
   return status_of(launch_pair(p));
 }

@@ -600,6 +600,25 @@ def test_linear_rows_that_start_on_any_value(m, n):
 
 @gpu
 @needs_cuda
+@pytest.mark.parametrize("m,n,k", [(500, 2567, 5040), (500, 2568, 5040), (300, 3882, 6160), (250, 2500, 9744), (250, 2496, 9744)])
+def test_linear_with_k_shared_by_several_pairs(m, n, k):
+    """Few tiles and a long K, shared unevenly by 2 to 4 pairs.  A part has no more blocks than the longest K above, and the
+    parts add at most three roundings of 6e-8: the same bars."""
+    g = gen(n + k)
+    _, codes, scales = lm_abi.rms_norm_quantize(torch.randn(m, k, generator=g, device="cuda"), norm=False)
+    w, ws = block_weight(g, n, k)
+    bias = torch.randn(n, generator=g, device="cuda").to(BF)
+    for dtype in (BF, torch.float32):
+        y, again = (torch.full((m, n), math.nan, dtype=dtype, device="cuda") for _ in range(2))
+        lm_abi.linear_block_fp8(codes, scales, w, ws, bias, y)
+        check_product(codes, scales, w, ws, bias, y)
+        lm_abi.linear_block_fp8(codes, scales, w, ws, bias, again)
+        assert torch.equal(y, again)
+    clean()
+
+
+@gpu
+@needs_cuda
 @pytest.mark.parametrize("m", [3, 40, 500])
 def test_linear_keeps_scales_apart_and_nan_in_its_row(m):
     """Scales of very different sizes (a block's partial product must not be rounded against another's), a NaN block."""
