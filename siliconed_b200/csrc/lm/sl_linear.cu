@@ -13,12 +13,12 @@
 //   memory by TMA stores, which run under the next tile's blocks.  What bounds it is a block's round trip through its TMEM
 //   buffer: 4 MMAs (650 cycles beside the epilogue's work), their commit (350), the partial read by 16 warps (450) and the
 //   buffer's release to the MMA threads (400), some 1900 cycles for the two buffers that 256 columns leave.  [4096, 3840] x
-//   [3840, 10240]: 182 us, 1770 TFLOP/s; without the epilogue's arithmetic 134 us, the loads take less.  (Tiles of 256 x
-//   128 with four buffers: 198 us, their MMAs read shared memory half again as often.  fma.rn.f32x2 for the sums: 293 us,
-//   pairs of registers moved together.  One issuing thread: 212 us.  The two halves of the columns issued by a thread
-//   each, two buffers each: 5 % slower, a is read twice.  16 epilogue warps of 64 columns: 258 us, spills.)  Where the
-//   tiles leave pairs idle, a cluster of up to 4 pairs shares a tile's K and adds its parts as below: [512, 9728] x [9728,
-//   2560] 24.7 us, 46.3 without.
+//   [3840, 10240]: 182 us, 1770 TFLOP/s (191 to 205 with inputs that change from call to call); without the epilogue's
+//   arithmetic 134 us, the loads take less.  (Beside the 182: tiles of 256 x 128 with four buffers 198 us, their MMAs read
+//   shared memory half again as often; fma.rn.f32x2 for the sums 293, pairs of registers moved together; one issuing
+//   thread 212; the two halves of the columns issued by a thread each, two buffers each, 5 % slower, a is read twice; 16
+//   epilogue warps of 64 columns 258, spills.)  Where the tiles leave pairs idle, a cluster of up to 4 pairs shares a
+//   tile's K and adds its parts as below: [512, 9728] x [9728, 2560] 24.7 us, 46.3 without.
 // - linear_swap: for few rows, bound by reading the weight.  The operands change places: 128 weight rows are the MMA's
 //   M and the rows of a, in tiles of up to 64, its N, so that no MMA row or TMEM column is padding; K is cut over the
 //   CTAs of a cluster, whose partials meet through distributed shared memory and are added in rank order.  The weight's
