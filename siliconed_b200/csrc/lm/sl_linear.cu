@@ -23,9 +23,9 @@
 //   M and the rows of a, in tiles of up to 64, its N, so that no MMA row or TMEM column is padding; K is cut over the
 //   CTAs of a cluster, whose partials meet through distributed shared memory and are added in rank order.  The weight's
 //   first tiles are prefetched to L2 while the kernel before this one ends.  One row of [4096, 12288] (from HBM, calls after
-//   one another): 12.0 us, 4.2 TB/s (0.65 of a copy's rate); 64 rows of it 17.8 us, 131 rows of [2560, 9728] 14.0 us: a block of
-//   64 rows keeps shared memory busy for some 640 cycles (its copies, the MMAs' operands, and the factors, which every
-//   thread reads 16 bytes at a time: without them 2.7 us less); eight epilogue warps spill and are slower.  (Room for a third
+//   one another): 12.0 us, 4.2 TB/s (0.65 of a copy's rate); 64 rows of it 17.0 us, 131 rows of [2560, 9728] 12.9 us, bound
+//   by the epilogue's instructions and by shared memory, which the copies, the MMAs' operands and the factors keep busy for some
+//   400 cycles a block of 64 rows; eight epilogue warps spill and are slower.  (Room for a third
 //   CTA an SM, so that the next call's begin early: 15.4 us for one row, the CTAs spread unevenly.)
 //
 // Rows past m or n and values past k arrive as zeros.  Every wait is bounded; no load uses cluster multicast.
@@ -73,16 +73,28 @@ __device__ __forceinline__ void tmem_wait(uint32_t (&r)[32]) {
                  "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
 }
 
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[8]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])::"memory");
+}
 __device__ __forceinline__ void tmem_wait(uint32_t (&r)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
                  "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
 }
-// 32 (16) consecutive fp32 columns of this thread's TMEM lane.
+// 32 consecutive fp32 columns of this thread's TMEM lane.
 __device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[32]) { sc::tmem_ld_32(taddr, r); }
-__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[16]) {
+// 16 (32) consecutive columns of 16 TMEM lanes, a warp's tile: a thread gets, of every 8 columns c and of the lanes from
+// `taddr` on, those of lane l / 4 in columns c + l % 4 * 2 and the next, and of lane l / 4 + 8 the same.
+__device__ __forceinline__ void tmem_load_tile(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_load_tile(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
       "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
@@ -482,6 +494,9 @@ static_assert(kMostRows * BN * 4 <= kRingBytes, "a partial fits the ring");
 // the epilogue to have read block g - kBuffers, so a stage must not come round sooner than a buffer.
 static_assert(kRingBytes / (kWBytes + kMostRows * kRowBytes) >= kBuffers && kMostStages >= kBuffers, "stages for the buffers");
 
+// Where column `col` of row `row` stands in shared memory.
+__device__ __forceinline__ int spread(int row, int col) { return col ^ (row >> 1 & 3) << 3; }
+
 // kRows: the sums' registers (16, 32 or 64); `rows` <= kRows is the tile's count, a multiple of 16, and the rows of
 // a's TMA box.
 template <bool kF32Out, int kRows>
@@ -576,16 +591,19 @@ __global__ void __launch_bounds__(kThreads, 2)
       sc::mbar_wait_drain(&s.drain[turn], 0);
     }
   } else {
-    // One column of y a thread.  The factors sa * sw come through shared memory, a group of blocks ahead of their use:
-    // thread t brings those of row t, lane i the weight's scale of block i.
+    // 4 columns of y a thread and a quarter of the rows.  The factors sa * sw come through shared memory, a group of blocks
+    // ahead of their use: thread t brings those of row t, lane i the weight's scale of block i.  (A column a thread and all
+    // rows: every thread reads all the factors, 13.9 us for 131 rows of [2560, 9728] where this takes
+    // 12.9; more columns or factors on their way at once 14.0 to 14.8.)
     const int et = threadIdx.x - kEpiWarp0 * 32, quarter = warp & 3;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     const float* sw = w_scales + static_cast<int64_t>(tile) * k_blocks;
     const bool owns = et < rows && m0 + et < m;
     const float* sa = a_scales + static_cast<int64_t>(owns ? m0 + et : 0) * k_blocks;
-    float acc[kRows], a_next[kGroup], w_next;
+    // Rows 8 g + l % 4 * 2 (+ 1), columns h * 16 + l / 4 (+ 8) of the warp's 32: sums [g][h][column * 2 + row].
+    float acc[kRows / 8][2][4], a_next[kGroup], w_next;
 #pragma unroll
-    for (int j = 0; j < kRows; ++j) acc[j] = 0.0f;
+    for (int j = 0; j < kRows; ++j) acc[j / 8][j / 4 % 2][j % 4] = 0.0f;
     const auto ask = [&](int kb) {
 #pragma unroll
       for (int i = 0; i < kGroup; ++i) a_next[i] = owns && kb + i < kb1 ? sa[kb + i] : 0.0f;
@@ -608,7 +626,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         ask(kb + kGroup);
         sc::named_barrier_sync(1, kEpiThreads);
       }
-      const float4* f = reinterpret_cast<const float4*>(factors[in_group]);
+      const float2* f = reinterpret_cast<const float2*>(factors[in_group]) + lane % 4;
       const bool ok = wait_warp(&s.done[stage], phase, abort, err, kSiteLinearSum);
       sc::tc_fence_after();
       if (ok) {
@@ -616,24 +634,26 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
         for (int q = 0; q < kRows; q += kChunk) {
           if (q >= rows) break;
-          uint32_t r[kChunk];
-          tmem_load(lanes + buf * kRows + q, r);
-          float4 v[kChunk / 4];
+          uint32_t r[2][kChunk / 2];
+          tmem_load_tile(lanes + buf * kRows + q, r[0]);
+          tmem_load_tile(lanes + (16u << 16) + buf * kRows + q, r[1]);
+          float2 v[kChunk / 8];
 #pragma unroll
-          for (int j = 0; j < kChunk / 4; ++j) v[j] = f[q / 4 + j];
-          tmem_wait(r);
+          for (int g = 0; g < kChunk / 8; ++g) v[g] = f[(q / 8 + g) * 4];
+          tmem_wait(r[0]);
+          tmem_wait(r[1]);
           if (q + kChunk >= rows) {  // all of the partial is in registers: its buffer is free
             sc::tc_fence_before();
             __syncwarp();
             if (lane == 0) sc::mbar_arrive(&s.part_empty[buf]);
           }
 #pragma unroll
-          for (int j = 0; j < kChunk; j += 4) {
-            acc[q + j] = fmaf(__uint_as_float(r[j]), v[j / 4].x, acc[q + j]);
-            acc[q + j + 1] = fmaf(__uint_as_float(r[j + 1]), v[j / 4].y, acc[q + j + 1]);
-            acc[q + j + 2] = fmaf(__uint_as_float(r[j + 2]), v[j / 4].z, acc[q + j + 2]);
-            acc[q + j + 3] = fmaf(__uint_as_float(r[j + 3]), v[j / 4].w, acc[q + j + 3]);
-          }
+          for (int g = 0; g < kChunk / 8; ++g)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              float& sum = acc[q / 8 + g][e / 4][e % 4];
+              sum = fmaf(__uint_as_float(r[e / 4][g * 4 + e % 4]), e % 2 == 0 ? v[g].x : v[g].y, sum);
+            }
         }
       }
       buf = buf + 1 == kBuffers ? 0 : buf + 1;
@@ -642,20 +662,28 @@ __global__ void __launch_bounds__(kThreads, 2)
         phase ^= 1u;
       }
     }
-    const int col = quarter * 32 + lane;
+    // In shared memory a row's columns are exchanged in groups of 8, so that a warp's 4 rows meet different banks.
+    const auto each = [&](auto&& put) {
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) {
+        const int g = j / 8, h = j / 4 % 2, e = j % 4;
+        const int row = g * 8 + lane % 4 * 2 + e % 2, col = quarter * 32 + h * 16 + lane / 4 + e / 2 * 8;
+        if (g * 8 < rows) put(row * BN + spread(row, col), acc[g][h][e], h * 2 + e / 2);
+      }
+    };
     if (parts == 1) {
       // Through shared memory (over the ring, as below), so that a warp's stores are of neighbours.  (Two bytes a lane straight
       // from the registers: 3900 cycles for 48 rows.)
-      const float add = bias_at(bias, n0 + col, n);
-      constexpr int kSize = kF32Out ? 4 : 2, kPer = 16 / kSize;  // bytes of a value, values of 16 bytes
+      float add[4];
 #pragma unroll
-      for (int j = 0; j < kRows; ++j)
-        if (j < rows) {
-          if (kF32Out)
-            reinterpret_cast<float*>(ring)[j * BN + col] = acc[j] + add;
-          else
-            reinterpret_cast<__nv_bfloat16*>(ring)[j * BN + col] = __float2bfloat16_rn(acc[j] + add);
-        }
+      for (int c = 0; c < 4; ++c) add[c] = bias_at(bias, n0 + quarter * 32 + lane / 4 + c * 8, n);
+      constexpr int kSize = kF32Out ? 4 : 2, kPer = 16 / kSize;  // bytes of a value, values of 16 bytes
+      each([&](int at, float sum, int c) {
+        if (kF32Out)
+          reinterpret_cast<float*>(ring)[at] = sum + add[c];
+        else
+          reinterpret_cast<__nv_bfloat16*>(ring)[at] = __float2bfloat16_rn(sum + add[c]);
+      });
       sc::named_barrier_sync(1, kEpiThreads);
       const int live = min(rows, m - m0);
       const bool wide = n % kPer == 0;  // rows of y start on 16 bytes
@@ -664,25 +692,22 @@ __global__ void __launch_bounds__(kThreads, 2)
           const int t = i / (BN / kPer), c = i % (BN / kPer) * kPer;
           if (n0 + c < n)
             *reinterpret_cast<uint4*>(static_cast<uint8_t*>(y) + (static_cast<int64_t>(m0 + t) * n + n0 + c) * kSize) =
-                *reinterpret_cast<const uint4*>(ring + (t * BN + c) * kSize);
+                *reinterpret_cast<const uint4*>(ring + (t * BN + spread(t, c)) * kSize);
         }
       } else if (n0 + et < n) {  // a value a lane, a row a step
 #pragma unroll 1
         for (int t = 0; t < live; ++t) {
           const int64_t at = static_cast<int64_t>(m0 + t) * n + n0 + et;
           if (kF32Out)
-            static_cast<float*>(y)[at] = reinterpret_cast<const float*>(ring)[t * BN + et];
+            static_cast<float*>(y)[at] = reinterpret_cast<const float*>(ring)[t * BN + spread(t, et)];
           else
-            static_cast<uint16_t*>(y)[at] = reinterpret_cast<const uint16_t*>(ring)[t * BN + et];
+            static_cast<uint16_t*>(y)[at] = reinterpret_cast<const uint16_t*>(ring)[t * BN + spread(t, et)];
         }
       }
     } else {
       // Over the ring: every copy has arrived and every MMA has read it, or the wait for the last partial gave up and
       // the kernel's error says so.
-      float* part = reinterpret_cast<float*>(ring);
-#pragma unroll
-      for (int j = 0; j < kRows; ++j)
-        if (j < rows) part[j * BN + col] = acc[j];
+      each([&](int at, float sum, int) { reinterpret_cast<float*>(ring)[at] = sum; });
     }
   }
   __syncwarp();
@@ -697,7 +722,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     const bool both = n % 2 == 0 && col + 1 < n;
     constexpr int kAdders = kThreads / (BN / 2);  // whole groups of threads
     for (int t = lo + group; group < kAdders && t < hi && m0 + t < m; t += kAdders) {
-      const float* mine = reinterpret_cast<const float*>(ring) + t * BN + 2 * cp;
+      const float* mine = reinterpret_cast<const float*>(ring) + t * BN + spread(t, 2 * cp);
       float2 sum = make_float2(0.0f, 0.0f);
       for (uint32_t q = 0; q < parts; ++q) {
         float2 v;
@@ -974,8 +999,8 @@ extern "C" int sl_linear_block_fp8(const uint8_t* a, const float* a_scales, cons
                   device.sms, encoder(), device.err, static_cast<cudaStream_t>(stream)};
   if (p.enc == nullptr || p.err == nullptr || p.sms < 2) return SL_CUDA_ERROR;
   // Up to 64 rows are always the few-rows kernel's; its row tiles are the grid's second dimension.  (Both measured, us, few-rows
-  // and many-rows kernel: [m, 2560] x [2560, 9728] 15.5 and 18.3 at 192 rows, 25.3 and 18.5 at 256, 29.1 and 31.3 at 384;
-  // [m, 4096] x [4096, 4096] 22.1 and 23.7 at 512, 43.5 and 24.3 at 640.)
+  // and many-rows kernel: [m, 2560] x [2560, 9728] 14.3 and 18.3 at 192 rows, 25.3 and 18.5 at 256, 29.1 and 31.3 at 384;
+  // [m, 4096] x [4096, 4096] 16.7 and 23.4 at 256, 22.1 and 19.4 at 512.)
   if (m <= swap::kMostRows || (m <= int64_t{65535} * swap::kMostRows &&
                                swap_plan(m, n, p.k_blocks, p.sms).us < pair_plan(m, n, p.k_blocks, p.sms).us))
     return status_of(p.f32 ? launch_swap<true>(p) : launch_swap<false>(p));
