@@ -14,7 +14,8 @@
 // context is cut between CTAs each writes its part's maximum, sum and unnormalised output to the workspace; the last to
 // arrive (a counter that it sets back to zero) adds the parts in the order of the shares, so every call gives the same
 // bits.  A CTA leaves at most two parts (its first and its last context), so the workspace does not grow with the batch.
-// (A queue that hands out the last quarter of the units in smaller pieces measured no faster.)
+// (A queue that hands out the last quarter of the units in smaller pieces measured no faster.  The share worked out and its
+// first unit brought to L2 while the kernel before this one ends: 2 % faster in a chain of long calls, 2 us slower alone.)
 //
 // Inside a CTA each warp takes steps of 32 tokens with a maximum, sum and output of its own, joined through shared
 // memory at the context's end.  Both products run on mma.sync m16n8k16 with the cache as the A operand:
