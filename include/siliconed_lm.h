@@ -105,6 +105,77 @@ SL_API int sl_linear_block_fp8(const uint8_t* a, const float* a_scales, const ui
                                const uint16_t* bias, int64_t m, int64_t n, int64_t k, void* y, int y_type,
                                void* stream);
 
+/*
+ * The same calls with their arguments in a struct, in the same order.  For callers to whom each argument of a foreign call
+ * costs: ctypes takes 2.7 us for 24 arguments, 0.7 us to pack and pass them at once.
+ */
+typedef struct {
+  const void* x;
+  int x_type;
+  const void* delta;
+  int delta_type;
+  const float* weight;
+  float eps;
+  int norm;
+  int64_t rows;
+  int d;
+  void* x_out;
+  uint8_t* codes;
+  float* scales;
+  void* stream;
+} sl_rms_norm_quantize_args;
+SL_API int sl_rms_norm_quantize_with(const sl_rms_norm_quantize_args* args);
+
+typedef struct {
+  const uint16_t* qkv;
+  int64_t tokens;
+  int heads, kv_heads, head_dim;
+  const float *norm_q, *norm_k;
+  float eps;
+  const float* freqs;
+  int max_pos, pairs;
+  const int32_t *seq, *positions, *table;
+  int seqs, table_width;
+  int64_t pages;
+  int page_size, cache_type;
+  void *k_cache, *v_cache;
+  float *k_scale, *v_scale;
+  uint16_t* q;
+  void* stream;
+} sl_append_paged_args;
+SL_API int sl_append_paged_with(const sl_append_paged_args* args);
+
+typedef struct {
+  const uint16_t* q;
+  const void *k_cache, *v_cache;
+  const float *k_scale, *v_scale;
+  int cache_type;
+  const int32_t *table, *lengths;
+  int batch, heads, kv_heads, head_dim, table_width;
+  int64_t pages;
+  int page_size;
+  float scale;
+  uint16_t* out;
+  float* lse;
+  void* workspace;
+  size_t workspace_bytes;
+  void* stream;
+} sl_paged_attention_args;
+SL_API int sl_paged_attention_with(const sl_paged_attention_args* args);
+
+typedef struct {
+  const uint8_t* a;
+  const float* a_scales;
+  const uint8_t* w;
+  const float* w_scales;
+  const uint16_t* bias;
+  int64_t m, n, k;
+  void* y;
+  int y_type;
+  void* stream;
+} sl_linear_block_fp8_args;
+SL_API int sl_linear_block_fp8_with(const sl_linear_block_fp8_args* args);
+
 /* Waits for the device, then reads and clears the library's error word on the current device: SL_TIMEOUT when a
  * bounded device-side wait gave up, SL_OUT_OF_RANGE when a page, position or sequence number was out of range
  * (the place in *site, which may be NULL), SL_CUDA_ERROR on an asynchronous CUDA error, else SL_OK. */

@@ -206,3 +206,10 @@ extern "C" int sl_append_paged(const uint16_t* qkv, int64_t tokens, int heads, i
   const bool halves = pairs == SL_PAIRS_HALVES;
   return status_of(head_dim == 64 ? launch_append<64>(a, halves, e4m3, st) : launch_append<128>(a, halves, e4m3, st));
 }
+
+extern "C" int sl_append_paged_with(const sl_append_paged_args* a) {
+  if (a == nullptr) return SL_INVALID_ARG;
+  return sl_append_paged(a->qkv, a->tokens, a->heads, a->kv_heads, a->head_dim, a->norm_q, a->norm_k, a->eps, a->freqs, a->max_pos,
+                         a->pairs, a->seq, a->positions, a->table, a->seqs, a->table_width, a->pages, a->page_size, a->cache_type,
+                         a->k_cache, a->v_cache, a->k_scale, a->v_scale, a->q, a->stream);
+}

@@ -845,3 +845,10 @@ extern "C" int sl_paged_attention(const uint16_t* q, const void* k_cache, const 
   }
   return SL_OK;
 }
+
+extern "C" int sl_paged_attention_with(const sl_paged_attention_args* a) {
+  if (a == nullptr) return SL_INVALID_ARG;
+  return sl_paged_attention(a->q, a->k_cache, a->v_cache, a->k_scale, a->v_scale, a->cache_type, a->table, a->lengths, a->batch,
+                            a->heads, a->kv_heads, a->head_dim, a->table_width, a->pages, a->page_size, a->scale, a->out, a->lse,
+                            a->workspace, a->workspace_bytes, a->stream);
+}

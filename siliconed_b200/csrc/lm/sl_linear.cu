@@ -1006,3 +1006,8 @@ extern "C" int sl_linear_block_fp8(const uint8_t* a, const float* a_scales, cons
     return status_of(p.f32 ? launch_swap<true>(p) : launch_swap<false>(p));
   return status_of(launch_pair(p));
 }
+
+extern "C" int sl_linear_block_fp8_with(const sl_linear_block_fp8_args* a) {
+  if (a == nullptr) return SL_INVALID_ARG;
+  return sl_linear_block_fp8(a->a, a->a_scales, a->w, a->w_scales, a->bias, a->m, a->n, a->k, a->y, a->y_type, a->stream);
+}

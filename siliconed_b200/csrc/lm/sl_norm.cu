@@ -133,3 +133,9 @@ extern "C" int sl_rms_norm_quantize(const void* x, int x_type, const void* delta
                 : (kind == 0 ? launch_norm<false, 0> : kind == 1 ? launch_norm<false, 1> : launch_norm<false, 2>);
   return status_of(go(x, delta, weight, eps, norm, rows, d, x_out, codes, scales, st));
 }
+
+extern "C" int sl_rms_norm_quantize_with(const sl_rms_norm_quantize_args* a) {
+  if (a == nullptr) return SL_INVALID_ARG;
+  return sl_rms_norm_quantize(a->x, a->x_type, a->delta, a->delta_type, a->weight, a->eps, a->norm, a->rows, a->d, a->x_out, a->codes,
+                              a->scales, a->stream);
+}

@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import os
 import re
+import struct
 
 import torch
 
@@ -33,8 +34,14 @@ SIGNATURES = {
     "sl_linear_block_fp8": (_I, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _P, _I, _P]),
     "sl_errors": (_I, [ctypes.POINTER(_I)]),
 }
+# The operators' calls with their arguments packed into a C struct: every argument of a ctypes call costs.
+_CODES = {_P: "P", _I: "i", _I64: "q", _F: "f", _SZ: "N"}
+_PACKED = {name: struct.Struct("@" + "".join(_CODES[t] for t in SIGNATURES[name][1]))
+           for name in ("sl_rms_norm_quantize", "sl_append_paged", "sl_paged_attention", "sl_linear_block_fp8")}
+SIGNATURES.update({name + "_with": (_I, [ctypes.c_char_p]) for name in _PACKED})
 
 _lib = None
+_calls: dict = {}
 
 
 class LmError(RuntimeError):
@@ -62,6 +69,7 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args
+    _calls.update({name: (getattr(lib, name + "_with"), form.pack) for name, form in _PACKED.items()})
     _lib = lib
     return lib
 
@@ -95,13 +103,18 @@ def _index(what: str, name: str, t, dims: int) -> int:
 
 
 def _call(fn: str, index: int, *args) -> None:
-    """The call on device `index` and its current stream."""
-    call = getattr(_lib or load(), fn)
-    if index == torch._C._cuda_getDevice():
-        status = call(*args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(index):
-            status = call(*args, torch._C._cuda_getCurrentRawStream(index))
+    """The call on device `index` and its current stream; a null pointer is 0."""
+    if _lib is None:
+        load()
+    call, pack = _calls[fn]
+    try:
+        if index == torch._C._cuda_getDevice():
+            status = call(pack(*args, torch._C._cuda_getCurrentRawStream(index)))
+        else:
+            with torch.cuda.device(index):
+                status = call(pack(*args, torch._C._cuda_getCurrentRawStream(index)))
+    except (struct.error, OverflowError) as e:
+        raise LmError(f"{fn}: {e}") from None
     if status != OK:
         raise LmError(f"{fn}: status {status}", status)
 
@@ -126,7 +139,7 @@ def rms_norm_quantize(x, delta=None, weight=None, eps: float = 1e-6, x_out=None,
     if x.dtype is not _F32 and x.dtype is not _BF16:
         _refuse(what, "x", x, (_BF16, _F32), shape, index)
     px = po = _take(what, "x", x, x.dtype, shape, index)
-    pd = pw = None
+    pd = pw = 0
     kind = BF16
     if delta is not None:
         kind = F32 if getattr(delta, "dtype", None) is _F32 else BF16
@@ -158,7 +171,7 @@ def _cache(what, k_cache, v_cache, k_scale, v_scale, index, kv_heads, head_dim):
         if k_scale is not None or v_scale is not None:
             raise LmError(f"{what}: a bf16 cache has no scales")
         return BF16, pages, size, _take(what, "k_cache", k_cache, _BF16, shape, index), \
-            _take(what, "v_cache", v_cache, _BF16, shape, index), None, None
+            _take(what, "v_cache", v_cache, _BF16, shape, index), 0, 0
     return E4M3, pages, size, _take(what, "k_cache", k_cache, _E4M3, shape, index), \
         _take(what, "v_cache", v_cache, _E4M3, shape, index), _take(what, "k_scale", k_scale, _F32, shape[:3], index), \
         _take(what, "v_scale", v_scale, _F32, shape[:3], index)
@@ -193,10 +206,10 @@ def append_paged(qkv, heads: int, kv_heads: int, norm_q, norm_k, eps: float, fre
     if q is None:
         q = torch.empty(tokens, heads, dim, dtype=_BF16, device=qkv.device)
     _call("sl_append_paged", index, _take(what, "qkv", qkv, _BF16, qkv.shape, index), tokens, heads, kv_heads, dim,
-          None if norm_q is None else _take(what, "norm_q", norm_q, _F32, (dim,), index),
-          None if norm_k is None else _take(what, "norm_k", norm_k, _F32, (dim,), index), eps,
+          0 if norm_q is None else _take(what, "norm_q", norm_q, _F32, (dim,), index),
+          0 if norm_k is None else _take(what, "norm_k", norm_k, _F32, (dim,), index), eps,
           _take(what, "freqs", freqs, _F32, (max_pos, dim // 2, 2), index), max_pos, PAIRS[pairs],
-          None if seq is None else _take(what, "seq", seq, _I32, (tokens,), index),
+          0 if seq is None else _take(what, "seq", seq, _I32, (tokens,), index),
           _take(what, "positions", positions, _I32, (tokens,), index), _take(what, "table", table, _I32, (seqs, width), index),
           seqs, width, pages, size, kind, pk, pv, pks, pvs, _take(what, "q", q, _BF16, (tokens, heads, dim), index))
     return q
@@ -256,7 +269,7 @@ def paged_attention(q, k_cache, v_cache, k_scale, v_scale, table, lengths, scale
     _call("sl_paged_attention", index, _take(what, "q", q, _BF16, shape, index), pk, pv, pks, pvs, kind,
           _take(what, "table", table, _I32, (batch, width), index), _take(what, "lengths", lengths, _I32, (batch,), index),
           batch, heads, kv_heads, dim, width, pages, size, scale, _take(what, "out", out, _BF16, shape, index),
-          None if lse is None else _take(what, "lse", lse, _F32, (batch, heads), index),
+          0 if lse is None else _take(what, "lse", lse, _F32, (batch, heads), index),
           _take(what, "workspace", workspace, torch.uint8, (space,), index), space)
     return out
 
@@ -280,7 +293,7 @@ def linear_block_fp8(codes, scales, weight, weight_scales, bias=None, out=None):
     _call("sl_linear_block_fp8", index, _take(what, "codes", codes, _E4M3, (m, k), index),
           _take(what, "scales", scales, _F32, (m, kb), index), _take(what, "weight", weight, _E4M3, (n, k), index),
           _take(what, "weight_scales", weight_scales, _F32, (nb, kb), index),
-          None if bias is None else _take(what, "bias", bias, _BF16, (n,), index), m, n, k,
+          0 if bias is None else _take(what, "bias", bias, _BF16, (n,), index), m, n, k,
           _take(what, "out", out, _F32 if kind == F32 else _BF16, (m, n), index), kind)
     return out
 

@@ -70,6 +70,22 @@ def test_null_and_bad_arguments_are_refused():
     assert lib.sl_paged_attention_workspace(4, 2, 128, None) == bad
 
 
+def test_packed_arguments_are_the_headers_structs():
+    """The packed calls' formats against the header: the same types in the same order, and no null struct taken."""
+    lib = lm_abi.load()
+    text = open(lm_abi.HEADER).read()
+    for name, form in lm_abi._PACKED.items():
+        body = text[:text.index("} " + name + "_args;")].rsplit("typedef struct {", 1)[1]
+        codes = ""
+        for member in body.strip().rstrip(";").split(";"):
+            base = member.replace("const", "").split()[0]
+            for field in member.split(","):
+                codes += "P" if "*" in field else {"int": "i", "int64_t": "q", "float": "f", "size_t": "N"}[base]
+        assert "@" + codes == form.format, name
+        assert getattr(lib, name + "_with")(None) == lm_abi.INVALID_ARG
+    assert lm_abi._PACKED["sl_rms_norm_quantize"].size % 8 == 0  # ends with the stream
+
+
 def test_wrappers_refuse_cpu_tensors():
     x = torch.zeros(2, 128)
     with pytest.raises(LmError):
