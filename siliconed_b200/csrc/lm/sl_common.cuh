@@ -34,6 +34,7 @@ constexpr float kScaleFloor = 1e-30f;
 
 // What a launch needs to know of the current device, asked of the runtime once per device.
 struct Device {
+  int index;
   int sms;   // its SMs; 0: the runtime gave an error
   int* err;  // the library's error word: [0] the code, [1] the site, [2] the block
 };

@@ -17,24 +17,24 @@ Device current_device() {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) {
     cudaGetLastError();
-    return {0, nullptr};
+    return {0, 0, nullptr};
   }
   if (dev < kDevices) {
     int* const word = g_words[dev].load(std::memory_order_acquire);
-    if (word != nullptr) return {g_sms[dev].load(std::memory_order_relaxed), word};
+    if (word != nullptr) return {dev, g_sms[dev].load(std::memory_order_relaxed), word};
   }
   int sms = 0;
   void* word = nullptr;
   if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
       cudaGetSymbolAddress(&word, g_errors) != cudaSuccess) {
     cudaGetLastError();
-    return {0, nullptr};
+    return {0, 0, nullptr};
   }
   if (dev < kDevices) {
     g_sms[dev].store(sms, std::memory_order_relaxed);
     g_words[dev].store(static_cast<int*>(word), std::memory_order_release);
   }
-  return {sms, static_cast<int*>(word)};
+  return {dev, sms, static_cast<int*>(word)};
 }
 
 }  // namespace sl

@@ -6,7 +6,7 @@
 // block's partial product in TMEM (tcgen05.mma kind::f8f6f4, four MMAs of K 32), and the epilogue warps multiply it
 // by its scales and add it to fp32 sums in registers while the MMAs of the next block run into the other TMEM buffer.
 //
-// Two kernels, by their estimated times (swap_plan(), pair_us()):
+// Two kernels, by their estimated times (swap_plan(), pair_plan()):
 //
 // - linear_pair: a cluster of two CTAs owns tiles of 256 x 256 of y (tcgen05.mma.cta_group::2), persistent over the
 //   tiles.  Each CTA loads its own 128 rows of a and of w by TMA (128-byte swizzle).  The tile leaves through shared
@@ -835,13 +835,8 @@ __global__ void __launch_bounds__(pair::kThreads, 1) seat_pair() {}
 // 8, and the first CTA past that starts a second wave (one row, k 5120 to 10240: 10.5 us up to 284 in clusters of 4,
 // 14.8 from 288).  The runtime is asked once per device and size.  0: it gave an error.
 template <bool kPair>
-int cluster_capacity(int c) {
+int cluster_capacity(int c, int dev) {
   static std::atomic<int> known[64][9];
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) {
-    cudaGetLastError();
-    return 0;
-  }
   if (dev < 64)
     if (const int n = known[dev][c].load(std::memory_order_relaxed); n != 0) return n;
   static unsigned long long configured = 0;
@@ -877,7 +872,7 @@ struct SwapPlan {
   int row_tiles, rows, parts;  // parts: of K, a cluster's CTAs
   double us;
 };
-SwapPlan swap_plan(int64_t m, int64_t n, int k_blocks, int sms) {
+SwapPlan swap_plan(int64_t m, int64_t n, int k_blocks, int sms, int dev) {
   SwapPlan s;
   s.row_tiles = static_cast<int>((m + swap::kMostRows - 1) / swap::kMostRows);
   s.rows = static_cast<int>(((m + s.row_tiles - 1) / s.row_tiles + 15) / 16 * 16);
@@ -885,7 +880,7 @@ SwapPlan swap_plan(int64_t m, int64_t n, int k_blocks, int sms) {
   s.parts = 1;
   s.us = 0.0;
   for (int c = 1; c <= 8 && c <= k_blocks; ++c) {
-    const int room = cluster_capacity<false>(c);
+    const int room = cluster_capacity<false>(c, dev);
     if (room == 0) continue;
     const double ctas = n_tiles * s.row_tiles * c, full = std::ceil(ctas / room) - 1.0, last = ctas - full * room;
     const auto blocks = [&](double at_once) {
@@ -905,13 +900,13 @@ struct PairPlan {
   int parts;
   double us;
 };
-PairPlan pair_plan(int64_t m, int64_t n, int k_blocks, int sms) {
+PairPlan pair_plan(int64_t m, int64_t n, int k_blocks, int sms, int dev) {
   const double n_tiles = static_cast<double>((n + pair::BN - 1) / pair::BN);
   const double tiles = static_cast<double>((m + 2 * pair::BM - 1) / (2 * pair::BM)) * n_tiles, waves = std::ceil(tiles / (sms / 2));
   const double bytes = n_tiles * k_blocks * 1.6e-3;
   PairPlan plan = {1, 6.3 + k_blocks * (0.63 * waves - 0.1) + bytes};
   for (int c = 2; c <= pair::kMostParts && c <= k_blocks && tiles * c <= sms / 2; ++c) {
-    if (tiles * 2 * c > cluster_capacity<true>(2 * c)) continue;
+    if (tiles * 2 * c > cluster_capacity<true>(2 * c, dev)) continue;
     const double us = 10.0 + (k_blocks + c - 1) / c * 0.53 + bytes;
     if (us < plan.us) plan = {c, us};
   }
@@ -919,7 +914,7 @@ PairPlan pair_plan(int64_t m, int64_t n, int k_blocks, int sms) {
 }
 
 template <bool kF32Out, bool kTmaOut>
-cudaError_t launch_pair_as(const Product& p) {
+cudaError_t launch_pair_as(const Product& p, int parts) {
   using namespace pair;
   auto kernel = linear_pair<kF32Out, kTmaOut>;
   static unsigned long long configured = 0;
@@ -937,22 +932,22 @@ cudaError_t launch_pair_as(const Product& p) {
     return cudaErrorInvalidValue;
   const int m_tiles = static_cast<int>((p.m + 2 * BM - 1) / (2 * BM)), n_tiles = static_cast<int>((p.n + BN - 1) / BN);
   const int64_t tiles = static_cast<int64_t>(m_tiles) * n_tiles;
-  const int parts = pair_plan(p.m, p.n, p.k_blocks, p.sms).parts;
   const int clusters = static_cast<int>(parts > 1 || tiles < p.sms / 2 ? tiles : p.sms / 2);
   return launch_cluster(kernel, dim3(static_cast<unsigned>(2 * parts * clusters)), kThreads, kSmemBytes, 2 * parts, p.stream, ta, tw,
                         ty, p.a_scales, p.w_scales, p.bias, p.y, static_cast<int>(p.m), static_cast<int>(p.n), p.k_blocks, m_tiles,
                         n_tiles, parts, p.err);
 }
 
-cudaError_t launch_pair(const Product& p) {
+cudaError_t launch_pair(const Product& p, int parts) {
   const bool tma = p.n % (p.f32 ? 4 : 8) == 0;
-  if (p.f32) return tma ? launch_pair_as<true, true>(p) : launch_pair_as<true, false>(p);
-  return tma ? launch_pair_as<false, true>(p) : launch_pair_as<false, false>(p);
+  if (p.f32) return tma ? launch_pair_as<true, true>(p, parts) : launch_pair_as<true, false>(p, parts);
+  return tma ? launch_pair_as<false, true>(p, parts) : launch_pair_as<false, false>(p, parts);
 }
 
 template <bool kF32Out, int kRows>
-cudaError_t launch_swap_as(const Product& p, int rows, int row_tiles) {
+cudaError_t launch_swap_as(const Product& p, const SwapPlan& plan) {
   using namespace swap;
+  const int rows = plan.rows, parts = plan.parts;
   auto kernel = linear_swap<kF32Out, kRows>;
   static unsigned long long configured = 0;
   if (const cudaError_t e = set_smem_once(kernel, static_cast<int>(kSmemBytes), configured); e != cudaSuccess) return e;
@@ -961,21 +956,18 @@ cudaError_t launch_swap_as(const Product& p, int rows, int row_tiles) {
       !make_map(&tw, p.enc, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.w, p.n, p.k, BN))
     return cudaErrorInvalidValue;
   const int64_t n_tiles = (p.n + BN - 1) / BN;
-  const int parts = swap_plan(p.m, p.n, p.k_blocks, p.sms).parts;
   int stages = kRingBytes / (kWBytes + rows * kRowBytes);
   if (stages > kMostStages) stages = kMostStages;
-  return launch_cluster(kernel, dim3(static_cast<unsigned>(n_tiles * parts), static_cast<unsigned>(row_tiles)),
+  return launch_cluster(kernel, dim3(static_cast<unsigned>(n_tiles * parts), static_cast<unsigned>(plan.row_tiles)),
                         kThreads, kSmemBytes, parts, p.stream, ta, tw, p.a_scales, p.w_scales, p.bias, p.y,
                         static_cast<int>(p.m), static_cast<int>(p.n), p.k_blocks, rows, stages, p.err);
 }
 
 template <bool kF32Out>
-cudaError_t launch_swap(const Product& p) {
-  const SwapPlan plan = swap_plan(p.m, p.n, p.k_blocks, p.sms);
-  const int rows = plan.rows, row_tiles = plan.row_tiles;
-  return rows <= 16    ? launch_swap_as<kF32Out, 16>(p, rows, row_tiles)
-         : rows <= 32  ? launch_swap_as<kF32Out, 32>(p, rows, row_tiles)
-                       : launch_swap_as<kF32Out, 64>(p, rows, row_tiles);
+cudaError_t launch_swap(const Product& p, const SwapPlan& plan) {
+  return plan.rows <= 16    ? launch_swap_as<kF32Out, 16>(p, plan)
+         : plan.rows <= 32  ? launch_swap_as<kF32Out, 32>(p, plan)
+                            : launch_swap_as<kF32Out, 64>(p, plan);
 }
 
 }  // namespace
@@ -1001,10 +993,13 @@ extern "C" int sl_linear_block_fp8(const uint8_t* a, const float* a_scales, cons
   // Up to 64 rows are always the few-rows kernel's; its row tiles are the grid's second dimension.  (Both measured, us, few-rows
   // and many-rows kernel: [m, 2560] x [2560, 9728] 14.3 and 18.3 at 192 rows, 25.3 and 18.5 at 256, 29.1 and 31.3 at 384;
   // [m, 4096] x [4096, 4096] 16.7 and 23.4 at 256, 22.1 and 19.4 at 512.)
-  if (m <= swap::kMostRows || (m <= int64_t{65535} * swap::kMostRows &&
-                               swap_plan(m, n, p.k_blocks, p.sms).us < pair_plan(m, n, p.k_blocks, p.sms).us))
-    return status_of(p.f32 ? launch_swap<true>(p) : launch_swap<false>(p));
-  return status_of(launch_pair(p));
+  PairPlan many = {1, 0.0};
+  if (m > swap::kMostRows) many = pair_plan(m, n, p.k_blocks, p.sms, device.index);
+  if (m <= int64_t{65535} * swap::kMostRows) {
+    const SwapPlan few = swap_plan(m, n, p.k_blocks, p.sms, device.index);
+    if (m <= swap::kMostRows || few.us < many.us) return status_of(p.f32 ? launch_swap<true>(p, few) : launch_swap<false>(p, few));
+  }
+  return status_of(launch_pair(p, many.parts));
 }
 
 extern "C" int sl_linear_block_fp8_with(const sl_linear_block_fp8_args* a) {
