@@ -167,8 +167,17 @@ struct Shape {
   static constexpr int kSmem = kWarps * kWarpBytes;
   static constexpr int kPartRow = kDim + 4;
   static constexpr int kPartFloats = kRows * (kDim + 2);
+  // A launch's shared memory on `workers` CTAs.  The ring also holds the factors of a cut context's parts when they are
+  // added, 8 bytes a row and part, and one context may be cut over every CTA: what the four-warp shapes' rings of 32 to 35 KB
+  // do not hold (592 parts of 8 rows: 37 KB).
+  static constexpr int smem_bytes(int workers) {
+    const int factors = kRows * workers * static_cast<int>(sizeof(float2));
+    return factors > kSmem ? factors : kSmem;
+  }
   static_assert(kRows * kPartRow * 4 <= kWarpBytes, "the join's part fits the ring");
   static_assert(!kE4m3 || kSlots % 2 == 0, "the scales go with whole steps");
+  // 6 KB a CTA beside the ring: the lengths, the first units, the joins' statistics and what the device keeps.
+  static_assert((smem_bytes(148 * kCtasPerSm) + 6 * 1024) * kCtasPerSm <= 227 * 1024, "a B200's SM holds its CTAs");
 };
 constexpr int kMostCtasPerSm = 4;
 
@@ -668,7 +677,7 @@ __global__ void __launch_bounds__(Shape<kDim, kE4m3, kNH, kWide>::kThreads, Shap
 #pragma unroll
         for (int w = 0; w < kEarly; ++w)
           if (w < count && tid / kRun < rows) early[w] = __ldcg(reinterpret_cast<const float4*>(part_of(w) + tid / kRun * kDim + d0));
-        float2* factor = reinterpret_cast<float2*>(ring);  // [rows][count]: m, then exp(m - top), and l
+        float2* factor = reinterpret_cast<float2*>(ring);  // [rows][count]: m, then exp(m - top), and l; see smem_bytes()
         for (int r = warp; r < rows; r += kWarps) {
           float top = -INFINITY;
           for (int w = lane; w < count; w += 32) {
@@ -729,9 +738,10 @@ template <int kDim, bool kE4m3, int kNH, bool kWide>
 cudaError_t launch_attention(const Attention& a, int sms, cudaStream_t stream) {
   using S = Shape<kDim, kE4m3, kNH, kWide>;
   auto kernel = paged_attention_k<kDim, kE4m3, kNH, kWide>;
-  static unsigned long long configured = 0;
-  if (const cudaError_t e = set_smem_once(kernel, S::kSmem, configured); e != cudaSuccess) return e;
-  return launch(kernel, dim3(static_cast<unsigned>(sms * S::kCtasPerSm)), dim3(S::kThreads), S::kSmem, stream, a);
+  const int workers = sms * S::kCtasPerSm, smem = S::smem_bytes(workers);
+  static unsigned long long configured = 0;  // a device's bytes are always the same; more than it has are refused
+  if (const cudaError_t e = set_smem_once(kernel, smem, configured); e != cudaSuccess) return e;
+  return launch(kernel, dim3(static_cast<unsigned>(workers)), dim3(S::kThreads), static_cast<size_t>(smem), stream, a);
 }
 
 template <int kDim, bool kE4m3>

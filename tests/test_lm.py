@@ -427,6 +427,36 @@ def test_attention_of_many_sequences():
 
 @gpu
 @needs_cuda
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("dim,heads", [(64, 8), (64, 7), (128, 8), (64, 16), (128, 16)])
+@pytest.mark.parametrize("long,others", [(80000, 0), (131072, 50)])
+def test_one_long_context_among_many_sequences(dim, heads, e4m3, long, others):
+    """One key-value head and 64 sequences of which one holds nearly all the tokens: its context is cut over nearly every
+    CTA of the launch, all of whose parts the last one to arrive adds."""
+    g = gen(dim + heads + others)
+    size, batch = 64, 64
+    lengths = [others] * batch
+    lengths[batch // 3] = long
+    width = -(-long // size)
+    pages = width + batch + 3
+    perm = torch.randperm(pages, generator=g, device="cuda").to(torch.int32)
+    table = torch.zeros(batch, width, dtype=torch.int32, device="cuda")
+    table[:, 0] = perm[width:width + batch]
+    table[batch // 3] = perm[:width]
+    k, v = make_cache(g, pages, 1, size, dim, e4m3)
+    q = (torch.randn(batch, heads, dim, generator=g, device="cuda") * 2).to(BF)
+    lens = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    lse, lse2 = torch.empty(batch, heads, device="cuda"), torch.empty(batch, heads, device="cuda")
+    scale = 1 / math.sqrt(dim)
+    out = lm_abi.paged_attention(q, k[0], v[0], k[1], v[1], table, lens, scale, lse=lse)
+    check_attention(q, k, v, table, lengths, scale, out, lse)
+    again = lm_abi.paged_attention(q, k[0], v[0], k[1], v[1], table, lens, scale, lse=lse2)
+    assert torch.equal(again, out) and torch.equal(lse, lse2)
+    clean()
+
+
+@gpu
+@needs_cuda
 @pytest.mark.parametrize("dim", [64, 128])
 def test_e4m3_cache_decodes_every_code(dim):
     """A context of one token gives its value row: all finite codes, exactly, in v and (as a sum of one) in k."""
