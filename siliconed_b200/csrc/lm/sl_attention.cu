@@ -39,6 +39,7 @@
 #include <cmath>
 
 #include "sl_common.cuh"
+#include "sl_ring.cuh"
 
 namespace sl {
 namespace {
@@ -204,7 +205,7 @@ __global__ void __launch_bounds__(Shape<kDim, kE4m3, kNH, kWide>::kThreads, Shap
   if (tid < kWarps * kSlots) sc::mbar_init(&arrived[0][0] + tid, 1);
   if (tid == 0) abort_flag = 0;
   sc::fence_mbar_init();
-  uint32_t fill = 0, take = 0, phases = 0;  // the warp's next slot to fill and to use, and the slots' parities
+  Ring<kSlots> order;  // of the warp's copies
   const uint32_t base = sc::smem_u32(ring) + warp * S::kWarpBytes;
   const uint8_t* const mine = ring + warp * S::kWarpBytes;
   sc::pdl_wait();
@@ -358,7 +359,7 @@ __global__ void __launch_bounds__(Shape<kDim, kE4m3, kNH, kWide>::kThreads, Shap
     };
     // The keys (values) of a step on their way into the next slot.
     auto next_slot = [&](const Tokens& k) {
-      uint64_t* bar = &arrived[warp][fill];
+      uint64_t* bar = &arrived[warp][order.fill];
       if (lane == 0) sc::mbar_arrive_expect_tx(bar, __popc(k.there) * kRowBytes);
       __syncwarp();
       return bar;
@@ -371,33 +372,36 @@ __global__ void __launch_bounds__(Shape<kDim, kE4m3, kNH, kWide>::kThreads, Shap
     };
     auto fetch_keys = [&](const Tokens& k) {
       uint64_t* bar = next_slot(k);
-      if (k.run != 0) copy(base + fill * S::kSlotBytes + lane * kRowBytes, a.k_cache, k.row, k.run, bar);
-      fill = fill + 1 == kSlots ? 0 : fill + 1;
+      if (k.run != 0) copy(base + order.fill * S::kSlotBytes + lane * kRowBytes, a.k_cache, k.row, k.run, bar);
+      order.filled();
     };
     auto fetch_values = [&](const Tokens& k) {
       uint64_t* bar = next_slot(k);
-      const uint32_t dst = base + fill * S::kSlotBytes + lane * kVPitch;
+      const uint32_t dst = base + order.fill * S::kSlotBytes + lane * kVPitch;
       if (S::kBig ? (k.there >> lane) & 1 : k.run != 0) copy(dst, a.v_cache, k.row, S::kBig ? 1 : k.run, bar);
       if (!((k.there >> lane) & 1)) {  // zeros where there is no token: p is 0 there, and 0 times anything finite is 0
         for (int i = 0; i < kRowBytes; i += 16)
           asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(dst + i), "r"(0) : "memory");
         sc::fence_async_shared();  // before a later copy into the slot
       }
-      fill = fill + 1 == kSlots ? 0 : fill + 1;
+      order.filled();
     };
-    // The oldest copy not yet used; null when it did not arrive in time.
+    // The oldest copy not yet used; null when it did not arrive in time: then it is still the oldest.
     auto arrival = [&]() -> const uint8_t* {
-      const bool ok = wait_warp(&arrived[warp][take], (phases >> take) & 1, &abort_flag, a.err, kSiteAttentionCopy);
-      const uint8_t* at = mine + take * S::kSlotBytes;
-      phases ^= 1u << take;
-      take = take + 1 == kSlots ? 0 : take + 1;
-      return ok ? at : nullptr;
+      if (!wait_warp(&arrived[warp][order.take], order.parity(), &abort_flag, a.err, kSiteAttentionCopy)) return nullptr;
+      const uint8_t* at = mine + order.take * S::kSlotBytes;
+      order.taken();
+      return at;
     };
 
     // Copy n is the keys of step n / 2 (n even) or its values (n odd); copy n + kSlots goes out when copy n has been used.
     // With an odd count of slots a step's keys go out before the values of the step before them.  Pages are looked up
     // one step before the copies need them.
-    const int t_first = t_begin + warp * kStep;
+    // Once a wait of the CTA has given up its warps take no more steps: a barrier whose phase has not ended is not armed again.
+    // The contexts' parts are written and counted all the same, so that the workspace is left ready.
+    const bool halted = __any_sync(0xFFFFFFFFu, *static_cast<volatile int*>(&abort_flag)) != 0;
+    const int t_first = halted ? t_end : t_begin + warp * kStep;
+    bool gave_up = false;
     uint32_t masks[kAhead + 1];  // of the tokens that are there, this step's first
     Tokens held = {0, 0, 0};
     int page = page_of(t_first), scale_slot = 0;
@@ -443,7 +447,7 @@ __global__ void __launch_bounds__(Shape<kDim, kE4m3, kNH, kWide>::kThreads, Shap
         for (int i = 0; i < 4; ++i) ks[i] = sc[g + 8 * i], vs[i] = sc[32 + g + 8 * i];
       }
       const uint8_t* const keys = arrival();
-      if (keys == nullptr) break;
+      if ((gave_up = keys == nullptr)) break;
       // S^T: tokens g + 8 i by query heads 2 c and 2 c + 1, in two MMA tiles.
       float s[kNH][2][4];
 #pragma unroll
@@ -545,7 +549,7 @@ __global__ void __launch_bounds__(Shape<kDim, kE4m3, kNH, kWide>::kThreads, Shap
                                                    : pack_bf16x2(x[2 * i], x[2 * i + 1]));
       }
       const uint8_t* const values = arrival();
-      if (values == nullptr) break;
+      if ((gave_up = values == nullptr)) break;
       // O^T += V^T P^T.  M tile i of load e: rows g are dims (8 e + g) kVDims + 2 i, rows g + 8 the dims after them.
 #pragma unroll
       for (int t = 0; t < 2; ++t)
@@ -595,13 +599,9 @@ __global__ void __launch_bounds__(Shape<kDim, kE4m3, kNH, kWide>::kThreads, Shap
       for (int i = 0; i < kAhead; ++i) masks[i] = masks[i + 1];
     }
     if (kE4m3) copy_wait<0>();
-    while (take != fill) {  // only after a wait that gave up: the copies still on their way
-      sc::mbar_wait_drain(&arrived[warp][take], (phases >> take) & 1);
-      phases ^= 1u << take;
-      take = take + 1 == kSlots ? 0 : take + 1;
-    }
+    if (gave_up) order.drain([&](uint32_t slot, uint32_t parity) { sc::mbar_wait_drain(&arrived[warp][slot], parity); });
 
-    // Join the warps.  Each writes its part over its own ring, whose copies have all arrived.
+    // Join the warps.  Each writes its part over its own ring, whose copies have all arrived (or were waited for twice).
     const float back = kE4m3 ? fmaxf(vtop, 7.9e-31f) * (1.0f / 32768.0f) : 1.0f;
     float* const part_o = reinterpret_cast<float*>(ring + warp * S::kWarpBytes);
     __syncwarp();

@@ -86,6 +86,61 @@ def test_packed_arguments_are_the_headers_structs():
     assert lm_abi._PACKED["sl_rms_norm_quantize"].size % 8 == 0  # ends with the stream
 
 
+def test_copies_in_flight_are_drained_after_a_wait_that_gave_up(tmp_path):
+    """The order of a warp's copies (sl_ring.cuh) on the host, against a model of the slots' barriers: whenever a wait gives
+    up, the drain waits for every copy still on its way, from the one that was waited for on, each with its phase's parity."""
+    (tmp_path / "ring.cc").write_text(r"""
+#include <cstdio>
+#include <deque>
+#include "sl_ring.cuh"
+template <int kSlots>
+bool run(unsigned seed, int ahead) {
+  for (int stop = 0; stop < 60; ++stop) {
+    sl::Ring<kSlots> order;
+    unsigned used[kSlots] = {}, random = seed * 7919u + stop;
+    std::deque<unsigned> flight;  // the slots of the copies on their way
+    unsigned next = 0;
+    for (int taken = 0;;) {
+      random = random * 1664525u + 1013904223u;
+      if (flight.size() < static_cast<size_t>(ahead) && (flight.empty() || random >> 31)) {
+        if (order.fill != next) return false;
+        flight.push_back(next);
+        next = (next + 1) % kSlots;
+        order.filled();
+        continue;
+      }
+      if (order.take != flight.front() || order.parity() != (used[flight.front()] & 1)) return false;
+      if (taken++ == stop) break;  // this wait gives up
+      ++used[flight.front()];
+      flight.pop_front();
+      order.taken();
+    }
+    bool good = true;
+    order.drain([&](uint32_t slot, uint32_t parity) {
+      good = good && !flight.empty() && slot == flight.front() && parity == (used[slot]++ & 1);
+      if (!flight.empty()) flight.pop_front();
+    });
+    if (!good || !flight.empty()) return false;
+  }
+  return true;
+}
+int main() {
+  for (unsigned seed = 0; seed < 50; ++seed)
+    for (int ahead = 1; ahead <= 8; ++ahead)
+      if ((ahead <= 2 && !run<2>(seed, ahead)) || (ahead <= 3 && !run<3>(seed, ahead)) || (ahead <= 4 && !run<4>(seed, ahead)) ||
+          !run<8>(seed, ahead))
+        return 1;
+  std::puts("ok");
+}
+""")
+    source = lm_abi.HERE + "/csrc/lm"
+    subprocess.run(["g++", "-std=c++17", "-I", source, "-x", "c++", str(tmp_path / "ring.cc"), "-o", str(tmp_path / "ring")], check=True)
+    assert subprocess.run([str(tmp_path / "ring")], capture_output=True, text=True).stdout == "ok\n"
+    # the attention keeps its copies in that order, and drains them where its waits give up
+    text = open(source + "/sl_attention.cu").read()
+    assert "Ring<kSlots> order" in text and "if (gave_up) order.drain(" in text and "phases ^=" not in text
+
+
 def test_wrappers_refuse_cpu_tensors():
     x = torch.zeros(2, 128)
     with pytest.raises(LmError):
