@@ -73,6 +73,7 @@ class PagedCache:
         self.k, self.v = (torch.zeros(shape, dtype=kind, device=device) for _ in range(2))
         self.k_scale, self.v_scale = (torch.zeros(shape[:4], device=device) for _ in range(2)) if e4m3 else (None, None)
         self.page_size = page_size
+        self.max_pos = cfg.max_pos  # the rotation table's rows: fewer than the table's slots where pages do not divide it
         self.width = -(-cfg.max_pos // page_size)
         self.table = torch.zeros(seqs, self.width, dtype=torch.int32, device=device)
         self.lengths = [0] * seqs
@@ -92,8 +93,8 @@ class PagedCache:
         need = [-(-(self.lengths[s] + count) // self.page_size) - len(self._pages[s]) for s in seqs]
         if sum(need) > len(self._free):
             raise LmError(f"PagedCache.extend: {sum(need)} pages wanted, {len(self._free)} free")
-        if any(self.lengths[s] + count > self.width * self.page_size for s in seqs):
-            raise LmError("PagedCache.extend: a sequence longer than the table")
+        if any(self.lengths[s] + count > self.max_pos for s in seqs):
+            raise LmError(f"PagedCache.extend: a sequence longer than {self.max_pos} positions")
         for s, n in zip(seqs, need):
             for _ in range(n):
                 page = self._free.pop()

@@ -39,6 +39,22 @@ def test_cache_hands_out_and_takes_back_pages():
         cache.admit()
 
 
+def test_cache_refuses_positions_past_the_rotation_table():
+    """Pages of 24 give 50 positions three pages, 72 slots: positions 50 .. have no row in the rotation table."""
+    from siliconed_b200.lm import DecoderConfig, PagedCache
+    from siliconed_b200.lm_abi import LmError
+    cfg = DecoderConfig(dim=256, hidden=512, heads=2, kv_heads=1, layers=1, max_pos=50)
+    cache = PagedCache(cfg, seqs=2, pages=8, page_size=24, device="cpu")
+    a, b = cache.admit(), cache.admit()
+    cache.extend([a, b], 49)
+    cache.extend([a])
+    with pytest.raises(LmError):
+        cache.extend([a])
+    with pytest.raises(LmError):
+        cache.extend([b], 2)
+    assert cache.lengths[a] == 50 and cache.lengths[b] == 49 and len(cache._free) == 2
+
+
 def test_weight_quantization_on_the_host():
     from siliconed_b200.lm import BlockWeight
     g = torch.Generator().manual_seed(0)
