@@ -80,15 +80,20 @@ class PagedCache:
         self._pages: list[list[int]] = [[] for _ in range(seqs)]
         self._free = list(range(pages - 1, -1, -1))
         self._unused = list(range(seqs - 1, -1, -1))
+        self._live: set[int] = set()
 
     def admit(self) -> int:
         """A sequence number for a new request."""
         if not self._unused:
             raise LmError("PagedCache.admit: every sequence is in use")
-        return self._unused.pop()
+        seq = self._unused.pop()
+        self._live.add(seq)
+        return seq
 
     def extend(self, seqs, count: int = 1) -> None:
         """Room for ``count`` more tokens of each sequence; the table's new entries go to the device in one copy."""
+        if count < 0 or len(set(seqs)) != len(seqs) or not self._live.issuperset(seqs):
+            raise LmError(f"PagedCache.extend: sequences in use, each once, and a count of 0 or more: got {seqs}, {count}")
         rows, columns, pages = [], [], []
         need = [-(-(self.lengths[s] + count) // self.page_size) - len(self._pages[s]) for s in seqs]
         if sum(need) > len(self._free):
@@ -109,6 +114,9 @@ class PagedCache:
 
     def release(self, seq: int) -> None:
         """The sequence's pages are free for others."""
+        if seq not in self._live:
+            raise LmError(f"PagedCache.release: sequence {seq} is not in use")
+        self._live.remove(seq)
         self._free.extend(reversed(self._pages[seq]))
         self._pages[seq] = []
         self.lengths[seq] = 0

@@ -55,6 +55,30 @@ def test_cache_refuses_positions_past_the_rotation_table():
     assert cache.lengths[a] == 50 and cache.lengths[b] == 49 and len(cache._free) == 2
 
 
+def test_cache_takes_sequences_in_use_once_each():
+    """A sequence named twice would get the pages of one extension for the length of two; one that is not in use, pages
+    that the next request admitted under its number would inherit."""
+    from siliconed_b200.lm import DecoderConfig, PagedCache
+    from siliconed_b200.lm_abi import LmError
+    cfg = DecoderConfig(dim=256, hidden=512, heads=2, kv_heads=1, layers=1, max_pos=64)
+    cache = PagedCache(cfg, seqs=3, pages=8, page_size=16, device="cpu")
+    a, b = cache.admit(), cache.admit()
+    cache.extend([a, b], 16)
+    unused = ({0, 1, 2} - {a, b}).pop()
+    for seqs, count in (([a, a], 16), ([a, b, a], 1), ([unused], 1), ([3], 1), ([-1], 1), ([a], -1)):
+        with pytest.raises(LmError):
+            cache.extend(seqs, count)
+    assert cache.lengths == [16 if s in (a, b) else 0 for s in range(3)] and len(cache._free) == 6
+    cache.release(a)
+    for seq in (a, unused, 3, -1):
+        with pytest.raises(LmError):
+            cache.release(seq)
+    assert len(cache._free) == 7 and sorted(cache._unused) == sorted((a, unused))
+    cache.extend([], 1)
+    cache.extend([b], 0)
+    assert cache.lengths[b] == 16
+
+
 def test_weight_quantization_on_the_host():
     from siliconed_b200.lm import BlockWeight
     g = torch.Generator().manual_seed(0)
