@@ -181,8 +181,9 @@ class Decoder:
         self.freqs = rotation_table(cfg, device)
 
     def forward(self, tokens, positions, table, lengths, cache: PagedCache, workspace=None):
-        """Logits fp32 [batch, vocab] of tokens int64 [batch] at positions int32 [batch]; table int32 [batch, width] and
-        lengths int32 [batch] (the new tokens counted) are the sequences' rows."""
+        """Logits fp32 [batch, vocab] of tokens int64 [batch], each below vocab (not checked here: they are on the device), at
+        positions int32 [batch]; table int32 [batch, width] and lengths int32 [batch] (the new tokens counted) are the
+        sequences' rows."""
         x, delta = self.embedding[tokens], None
         for i, layer in enumerate(self.layers):
             delta = layer.forward(x, delta, self.freqs, positions, table, lengths, cache.layer(i), workspace)
@@ -191,6 +192,9 @@ class Decoder:
 
     def step(self, tokens: list[int], seqs: list[int], cache: PagedCache):
         """Appends one token to each sequence and returns its logits."""
+        # an index past the embedding is a failed assertion on the device, which ends the process's CUDA context
+        if len(tokens) != len(seqs) or not all(0 <= t < self.cfg.vocab for t in tokens):
+            raise LmError(f"Decoder.step: a token below {self.cfg.vocab} for each sequence: got {tokens} for {seqs}")
         cache.extend(seqs)
         lengths = torch.tensor([cache.lengths[s] for s in seqs], dtype=torch.int32).to(self.device)
         rows = torch.tensor(seqs).to(self.device)

@@ -79,6 +79,21 @@ def test_cache_takes_sequences_in_use_once_each():
     assert cache.lengths[b] == 16
 
 
+def test_step_refuses_tokens_that_the_embedding_does_not_have():
+    """Refused on the host, before anything reaches the cache or the device (there an index out of range is an assertion)."""
+    from siliconed_b200.lm import Decoder, DecoderConfig, PagedCache
+    from siliconed_b200.lm_abi import LmError
+    cfg = DecoderConfig(dim=256, hidden=512, heads=2, kv_heads=1, layers=1, vocab=300, max_pos=64)
+    cache = PagedCache(cfg, seqs=2, pages=8, page_size=16, device="cpu")
+    model = Decoder.__new__(Decoder)  # the configuration alone: nothing else may be looked at
+    model.cfg = cfg
+    a, b = cache.admit(), cache.admit()
+    for tokens, seqs in (([300, 0], [a, b]), ([0, -1], [a, b]), ([0], [a, b]), ([0, 1], [a])):
+        with pytest.raises(LmError):
+            model.step(tokens, seqs, cache)
+    assert cache.lengths == [0, 0] and len(cache._free) == 8
+
+
 def test_weight_quantization_on_the_host():
     from siliconed_b200.lm import BlockWeight
     g = torch.Generator().manual_seed(0)
