@@ -184,7 +184,7 @@ extern "C" int sl_append_paged(const uint16_t* qkv, int64_t tokens, int heads, i
   using namespace sl;
   if (tokens < 0 || tokens > 0x7FFFFFFF || heads < 1 || kv_heads < 1 || heads > 65536 || kv_heads > 65536 ||
       (head_dim != 64 && head_dim != 128) || max_pos < 1 ||
-      (pairs != SL_PAIRS_ADJACENT && pairs != SL_PAIRS_HALVES) || seqs < 1 || table_width < 1 || pages < 1 ||
+      (pairs != SL_PAIRS_ADJACENT && pairs != SL_PAIRS_HALVES) || seqs < 0 || (seqs == 0 && tokens != 0) || table_width < 1 || pages < 1 ||
       page_size < 1 || (cache_type != SL_BF16 && cache_type != SL_E4M3))
     return SL_INVALID_ARG;
   if (seq == nullptr && tokens > seqs) return SL_INVALID_ARG;

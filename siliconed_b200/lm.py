@@ -195,6 +195,8 @@ class Decoder:
         # an index past the embedding is a failed assertion on the device, which ends the process's CUDA context
         if len(tokens) != len(seqs) or not all(0 <= t < self.cfg.vocab for t in tokens):
             raise LmError(f"Decoder.step: a token below {self.cfg.vocab} for each sequence: got {tokens} for {seqs}")
+        if not seqs:
+            return torch.empty(0, self.cfg.vocab, device=self.device)
         cache.extend(seqs)
         lengths = torch.tensor([cache.lengths[s] for s in seqs], dtype=torch.int32).to(self.device)
         rows = torch.tensor(seqs).to(self.device)

@@ -199,7 +199,7 @@ def append_paged(qkv, heads: int, kv_heads: int, norm_q, norm_k, eps: float, fre
     if not isinstance(freqs, torch.Tensor) or freqs.dim() != 3 or not isinstance(table, torch.Tensor) or table.dim() != 2:
         raise LmError(f"{what}: freqs must be [max_pos, head_dim / 2, 2], table [seqs, width]")
     max_pos, (seqs, width) = freqs.shape[0], table.shape
-    if max_pos == 0 or seqs == 0 or width == 0:
+    if max_pos == 0 or width == 0 or (seqs == 0 and tokens != 0):
         raise LmError(f"{what}: an empty table or freqs")
     if seq is None and tokens > seqs:
         raise LmError(f"{what}: {tokens} tokens for {seqs} sequences")

@@ -86,6 +86,35 @@ def test_packed_arguments_are_the_headers_structs():
     assert lm_abi._PACKED["sl_rms_norm_quantize"].size % 8 == 0  # ends with the stream
 
 
+def test_nothing_to_do_is_a_no_op():
+    """Zero rows, tokens or sequences, the append's table of no sequences among them; pointers are not looked at."""
+    lib = lm_abi.load()
+    assert lib.sl_append_paged(None, 0, 4, 2, 128, None, None, 1e-6, None, 16, 0, None, None, None, 0, 4, 8, 16, 0, None, None,
+                               None, None, None, None) == lm_abi.OK
+    assert lib.sl_append_paged(None, 0, 4, 2, 128, None, None, 1e-6, None, 16, 0, None, None, None, -1, 4, 8, 16, 0, None, None,
+                               None, None, None, None) == lm_abi.INVALID_ARG
+    assert lib.sl_paged_attention(None, None, None, None, None, 0, None, None, 0, 4, 2, 128, 4, 8, 16, 0.1, None, None, None, 0,
+                                  None) == lm_abi.OK
+    assert lib.sl_linear_block_fp8(None, None, None, None, None, 0, 128, 256, None, 0, None) == lm_abi.OK
+
+
+@gpu
+@needs_cuda
+def test_wrappers_of_no_sequences():
+    def table(*shape):
+        return torch.zeros(shape, dtype=torch.int32, device="cuda")
+
+    kc, vc = (torch.zeros(4, 2, 16, 128, dtype=BF, device="cuda") for _ in range(2))
+    qkv = torch.zeros(0, 8 * 128, dtype=BF, device="cuda")
+    q = lm_abi.append_paged(qkv, 4, 2, None, None, 1e-6, rope_table(16, 128), "halves", None, table(0), table(0, 3), kc, vc)
+    assert q.shape == (0, 4, 128)
+    assert lm_abi.paged_attention(q, kc, vc, None, None, table(0, 3), table(0), 0.1).shape == (0, 4, 128)
+    with pytest.raises(LmError):
+        lm_abi.append_paged(torch.zeros(1, 8 * 128, dtype=BF, device="cuda"), 4, 2, None, None, 1e-6, rope_table(16, 128), "halves",
+                            table(1), table(1), table(0, 3), kc, vc)
+    clean()
+
+
 def test_copies_in_flight_are_drained_after_a_wait_that_gave_up(tmp_path):
     """The order of a warp's copies (sl_ring.cuh) on the host, against a model of the slots' barriers: whenever a wait gives
     up, the drain waits for every copy still on its way, from the one that was waited for on, each with its phase's parity."""

@@ -94,6 +94,15 @@ def test_step_refuses_tokens_that_the_embedding_does_not_have():
     assert cache.lengths == [0, 0] and len(cache._free) == 8
 
 
+def test_step_of_no_sequences():
+    from siliconed_b200.lm import Decoder, DecoderConfig, PagedCache
+    cfg = DecoderConfig(dim=256, hidden=512, heads=2, kv_heads=1, layers=1, vocab=300, max_pos=64)
+    model = Decoder.__new__(Decoder)
+    model.cfg, model.device = cfg, torch.device("cpu")
+    logits = model.step([], [], PagedCache(cfg, seqs=2, pages=8, page_size=16, device="cpu"))
+    assert logits.shape == (0, 300) and logits.dtype == torch.float32
+
+
 def test_weight_quantization_on_the_host():
     from siliconed_b200.lm import BlockWeight
     g = torch.Generator().manual_seed(0)
