@@ -115,6 +115,13 @@ __device__ __forceinline__ void bulk_wait_read() {
 }
 __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
+// A barrier of the cluster's threads.  The instructions are the aligned ones, which all of a warp must reach together: lanes
+// that a loop or a guarded store parted come together first.
+__device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
+  sc::cluster_barrier();
+}
+
 __device__ __forceinline__ float bias_at(const uint16_t* bias, int col, int n) {
   return bias != nullptr && col < n ? from_bf16(bias[col]) : 0.0f;
 }
@@ -192,7 +199,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   __syncwarp();
   sc::tc_fence_before();
-  sc::cluster_barrier();
+  cluster_sync();
   sc::tc_fence_after();
   const uint32_t tmem = s.tmem_base;
   sc::pdl_wait();
@@ -341,7 +348,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (kTmaOut && lane == 0) bulk_wait_all();
     if (parts > 1) {
       // Every part's pair adds a share of the rows, in the parts' order: the same sums whichever adds them.
-      sc::cluster_barrier();
+      cluster_sync();
       int mt, nt;
       sc::tile_coords(first, m_tiles, n_tiles, mt, nt);
       const int row0 = (mt * 2 + static_cast<int>(rank)) * BM;
@@ -450,12 +457,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     __syncwarp();
-    if (parts > 1) sc::cluster_barrier();
+    if (parts > 1) cluster_sync();
   }
   // No CTA leaves while the pair's MMAs, TMEM or barriers or the cluster's sums may still reach its memory.
   __syncwarp();
   sc::tc_fence_before();
-  sc::cluster_barrier();
+  cluster_sync();
   if (warp == 1) {
     sc::tc_fence_after();
     sc::tmem_dealloc_pair(tmem, kTmemCols);
@@ -714,7 +721,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   sc::tc_fence_before();
   if (parts > 1) {
     // Every CTA adds a share of the rows, in rank order: the same sums whichever CTA adds them.
-    sc::cluster_barrier();
+    cluster_sync();
     const int cp = threadIdx.x % (BN / 2), group = threadIdx.x / (BN / 2);
     const int lo = static_cast<int>(rank) * rows / static_cast<int>(parts), hi = static_cast<int>(rank + 1) * rows / static_cast<int>(parts);
     const int col = n0 + 2 * cp;
@@ -751,7 +758,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
       }
     }
-    sc::cluster_barrier();  // the partials stay until the other CTAs have read them
+    cluster_sync();  // the partials stay until the other CTAs have read them
   } else {
     __syncthreads();
   }

@@ -115,6 +115,13 @@ def test_wrappers_of_no_sequences():
     clean()
 
 
+def test_warps_come_together_before_a_cluster_barrier():
+    """The aligned barrier instructions are undefined for a warp whose lanes are apart."""
+    text = open(lm_abi.HERE + "/csrc/lm/sl_linear.cu").read()
+    assert text.count("cluster_barrier()") == 1 and "  __syncwarp();\n  sc::cluster_barrier();" in text
+    assert text.count("cluster_sync();") >= 5
+
+
 def test_copies_in_flight_are_drained_after_a_wait_that_gave_up(tmp_path):
     """The order of a warp's copies (sl_ring.cuh) on the host, against a model of the slots' barriers: whenever a wait gives
     up, the drain waits for every copy still on its way, from the one that was waited for on, each with its phase's parity."""
