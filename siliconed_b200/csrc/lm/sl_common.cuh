@@ -63,7 +63,9 @@ cudaError_t set_smem_once(Kernel kernel, int bytes, unsigned long long& done) {
 
 // A launch whose set-up may overlap the end of the kernel before it on the stream.  Every kernel launched so
 // executes griddepcontrol.wait in every thread before its first global access, and so orders itself after
-// everything its predecessor was ordered after.
+// everything its predecessor was ordered after.  What that predecessor wrote changes while this kernel is already running, so
+// no pointer is __restrict__ const and no load a read-only one (ld.global.nc): those promise values that stay the same for the
+// kernel's whole life.
 template <typename... Params, typename... Args>
 cudaError_t launch(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
   cudaLaunchConfig_t cfg = {};

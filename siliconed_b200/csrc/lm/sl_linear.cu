@@ -164,8 +164,8 @@ static_assert(BM * kPartRow <= 2 * kStages * kTileBytes, "a part's sums fit the 
 template <bool kF32Out, bool kTmaOut>
 __global__ void __launch_bounds__(kThreads, 1)
     linear_pair(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_w,
-                const __grid_constant__ CUtensorMap tm_y, const float* __restrict__ a_scales,
-                const float* __restrict__ w_scales, const uint16_t* __restrict__ bias, void* __restrict__ y, int m, int n,
+                const __grid_constant__ CUtensorMap tm_y, const float* a_scales,
+                const float* w_scales, const uint16_t* bias, void* y, int m, int n,
                 int k_blocks, int m_tiles, int n_tiles, int parts, int* err) {
   extern __shared__ uint8_t smem_raw[];
   Smem& s = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -509,8 +509,8 @@ __device__ __forceinline__ int spread(int row, int col) { return col ^ (row >> 1
 template <bool kF32Out, int kRows>
 __global__ void __launch_bounds__(kThreads, 2)
     linear_swap(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_w,
-                const float* __restrict__ a_scales, const float* __restrict__ w_scales,
-                const uint16_t* __restrict__ bias, void* __restrict__ y, int m, int n, int k_blocks, int rows, int stages,
+                const float* a_scales, const float* w_scales,
+                const uint16_t* bias, void* y, int m, int n, int k_blocks, int rows, int stages,
                 int* err) {
   constexpr uint32_t kTmemCols = kBuffers * kRows;
   extern __shared__ uint8_t smem_raw[];

@@ -122,6 +122,16 @@ def test_warps_come_together_before_a_cluster_barrier():
     assert text.count("cluster_sync();") >= 5
 
 
+def test_no_load_is_promised_to_be_constant():
+    """The kernels start before the one ahead of them has written their inputs: a read-only load may be moved above the wait."""
+    import glob
+    import re
+    for path in glob.glob(lm_abi.HERE + "/csrc/lm/*"):
+        code = re.sub(r"//[^\n]*", "", open(path).read())
+        for word in ("__restrict", "__ldg", "global.nc"):
+            assert word not in code, (path, word)
+
+
 def test_copies_in_flight_are_drained_after_a_wait_that_gave_up(tmp_path):
     """The order of a warp's copies (sl_ring.cuh) on the host, against a model of the slots' barriers: whenever a wait gives
     up, the drain waits for every copy still on its way, from the one that was waited for on, each with its phase's parity."""
