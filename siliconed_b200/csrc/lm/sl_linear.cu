@@ -720,8 +720,9 @@ __global__ void __launch_bounds__(kThreads, 2)
   __syncwarp();
   sc::tc_fence_before();
   if (parts > 1) {
-    // Every CTA adds a share of the rows, in rank order: the same sums whichever CTA adds them.
-    cluster_sync();
+    // Every CTA adds a share of the rows, in rank order: the same sums whichever CTA adds them.  (The warps are together; a
+    // second __syncwarp() here: 12.3 us for one row of [4096, 12288], 12.05 without.)
+    sc::cluster_barrier();
     const int cp = threadIdx.x % (BN / 2), group = threadIdx.x / (BN / 2);
     const int lo = static_cast<int>(rank) * rows / static_cast<int>(parts), hi = static_cast<int>(rank + 1) * rows / static_cast<int>(parts);
     const int col = n0 + 2 * cp;
