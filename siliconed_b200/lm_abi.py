@@ -265,7 +265,7 @@ def paged_attention(q, k_cache, v_cache, k_scale, v_scale, table, lengths, scale
         out = torch.empty_like(q)
     if workspace is None:
         workspace = _stream_workspace(heads, kv_heads, dim, index)
-    space = workspace.numel()
+    space = workspace.numel() if isinstance(workspace, torch.Tensor) else 0
     _call("sl_paged_attention", index, _take(what, "q", q, _BF16, shape, index), pk, pv, pks, pvs, kind,
           _take(what, "table", table, _I32, (batch, width), index), _take(what, "lengths", lengths, _I32, (batch,), index),
           batch, heads, kv_heads, dim, width, pages, size, scale, _take(what, "out", out, _BF16, shape, index),

@@ -100,6 +100,20 @@ def test_nothing_to_do_is_a_no_op():
 
 @gpu
 @needs_cuda
+def test_attention_refuses_a_workspace_that_does_not_fit():
+    q = torch.zeros(2, 4, 128, dtype=BF, device="cuda")
+    cache = torch.zeros(4, 2, 16, 128, dtype=BF, device="cuda")
+    table, lens = torch.zeros(2, 2, dtype=torch.int32, device="cuda"), torch.ones(2, dtype=torch.int32, device="cuda")
+    good = lm_abi.attention_workspace(4, 2, 128)
+    for bad in (1 << 24, good.cpu(), good.float(), good[:-16], good[::2]):
+        with pytest.raises(LmError):
+            lm_abi.paged_attention(q, cache, cache, None, None, table, lens, 0.1, workspace=bad)
+    lm_abi.paged_attention(q, cache, cache, None, None, table, lens, 0.1, workspace=good)
+    clean()
+
+
+@gpu
+@needs_cuda
 def test_wrappers_of_no_sequences():
     def table(*shape):
         return torch.zeros(shape, dtype=torch.int32, device="cuda")
