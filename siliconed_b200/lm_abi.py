@@ -216,6 +216,7 @@ def append_paged(qkv, heads: int, kv_heads: int, norm_q, norm_k, eps: float, fre
 
 
 _workspaces: dict = {}
+_MOST_WORKSPACES = 16  # 2 to 10 MB each
 
 
 def attention_workspace(heads: int, kv_heads: int, head_dim: int, device=None):
@@ -230,13 +231,16 @@ def attention_workspace(heads: int, kv_heads: int, head_dim: int, device=None):
 
 
 def _stream_workspace(heads, kv_heads, dim, index):
-    """The current stream's workspace.  A call under graph capture gets one of its own, zeroed inside the graph: memory
-    that only a replay writes must not be handed to later calls."""
+    """The current stream's workspace, of which the latest few are kept: a program may make streams as it goes.  (One that is
+    dropped goes back to the allocator for its own stream, behind the calls that use it.)  A call under graph capture gets one
+    of its own, zeroed inside the graph: memory that only a replay writes must not be handed to later calls."""
     if torch.cuda.is_current_stream_capturing():
         return attention_workspace(heads, kv_heads, dim, index)
     key = (index, torch._C._cuda_getCurrentRawStream(index), heads > 8 * kv_heads, dim)
     ws = _workspaces.get(key)
     if ws is None:
+        while len(_workspaces) >= _MOST_WORKSPACES:
+            _workspaces.pop(next(iter(_workspaces)), None)
         ws = _workspaces[key] = attention_workspace(heads, kv_heads, dim, index)
     return ws
 

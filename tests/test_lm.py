@@ -112,6 +112,23 @@ def test_attention_refuses_a_workspace_that_does_not_fit():
     clean()
 
 
+def test_few_workspaces_are_kept(monkeypatch):
+    """One a stream and kind for streams in use, but not one for every stream that ever was."""
+    stream = [0]
+    monkeypatch.setattr(lm_abi, "_workspaces", {})
+    monkeypatch.setattr(lm_abi, "attention_workspace", lambda *a: object())
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: stream[0], raising=False)
+    kinds = [(8, 1, 64), (8, 1, 128), (16, 1, 64), (16, 1, 128)]
+    first = [lm_abi._stream_workspace(*kind, 0) for kind in kinds]
+    assert len({id(w) for w in first}) == 4
+    assert all(lm_abi._stream_workspace(*kind, 0) is w for kind, w in zip(kinds, first))
+    for stream[0] in range(1, 100):
+        one = lm_abi._stream_workspace(8, 1, 64, 0)
+        assert lm_abi._stream_workspace(8, 1, 64, 0) is one
+    assert len(lm_abi._workspaces) == lm_abi._MOST_WORKSPACES
+
+
 @gpu
 @needs_cuda
 def test_wrappers_of_no_sequences():
