@@ -322,21 +322,10 @@ __global__ void __launch_bounds__(Shape<kDim, kE4m3, kNH, kWide>::kThreads, Shap
       for (int i = 0; i < kPairs; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.0f;
     }
 
-    // The page of token t + lane (-1: none), asked for one step before it is used, and its cache row, all ones where
-    // there is none.
+    // The page of token t + lane (-1: none), asked for one step before it is used.
     auto page_of = [&](int t) -> int {
       t += lane;
       return t < t_end ? table[a.page_shift >= 0 ? t >> a.page_shift : t / a.page_size] : -1;
-    };
-    auto row_of = [&](int t, int page) -> uint32_t {
-      t += lane;
-      if (t >= t_end) return 0xFFFFFFFFu;
-      if (page < 0 || page >= a.pages) {
-        sc::record_error(a.err, kErrRange, kSiteAttentionPage);
-        return 0xFFFFFFFFu;
-      }
-      return (static_cast<uint32_t>(page) * a.kv_heads + kvh) * a.page_size +
-             (a.page_shift >= 0 ? t & (a.page_size - 1) : t % a.page_size);
     };
     // The tokens of a step, one a lane: its cache row, whether there is one (`there` is the mask of all lanes), and the
     // count of rows that follow one another in the cache from here on (0 inside such a run).
