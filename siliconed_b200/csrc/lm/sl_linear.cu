@@ -478,8 +478,8 @@ namespace swap {
 constexpr int BN = 128;                   // rows of w (columns of y) a CTA
 constexpr int kMostRows = 64;            // rows of a, the MMA's N
 constexpr int kWBytes = BN * kRowBytes;
-constexpr int kMostStages = 6;
 constexpr int kRingBytes = 100 * 1024;    // two CTAs an SM
+constexpr int kMostStages = kRingBytes / (kWBytes + 16 * kRowBytes);  // 5: of 16 rows, and of 32; 4 of 48 and 64
 constexpr int kGroup = 8;                 // blocks whose factors are brought in together
 constexpr int kBuffers = 4;               // partial products in TMEM
 constexpr int kEpiWarp0 = 3, kEpiWarps = 4, kEpiThreads = kEpiWarps * 32;
@@ -499,7 +499,7 @@ static_assert(kEpiThreads == BN, "a thread per column");
 static_assert(kMostRows * BN * 4 <= kRingBytes, "a partial fits the ring");
 // Every wait's parity tells one phase from the next as long as nobody is two phases ahead: the MMAs of block g wait for
 // the epilogue to have read block g - kBuffers, so a stage must not come round sooner than a buffer.
-static_assert(kRingBytes / (kWBytes + kMostRows * kRowBytes) >= kBuffers && kMostStages >= kBuffers, "stages for the buffers");
+static_assert(kRingBytes / (kWBytes + kMostRows * kRowBytes) >= kBuffers, "stages for the buffers");
 
 // Where column `col` of row `row` stands in shared memory.
 __device__ __forceinline__ int spread(int row, int col) { return col ^ (row >> 1 & 3) << 3; }
@@ -964,8 +964,7 @@ cudaError_t launch_swap_as(const Product& p, const SwapPlan& plan) {
       !make_map(&tw, p.enc, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.w, p.n, p.k, BN))
     return cudaErrorInvalidValue;
   const int64_t n_tiles = (p.n + BN - 1) / BN;
-  int stages = kRingBytes / (kWBytes + rows * kRowBytes);
-  if (stages > kMostStages) stages = kMostStages;
+  const int stages = kRingBytes / (kWBytes + rows * kRowBytes);  // rows are 16 at least
   return launch_cluster(kernel, dim3(static_cast<unsigned>(n_tiles * parts), static_cast<unsigned>(plan.row_tiles)),
                         kThreads, kSmemBytes, parts, p.stream, ta, tw, p.a_scales, p.w_scales, p.bias, p.y,
                         static_cast<int>(p.m), static_cast<int>(p.n), p.k_blocks, rows, stages, p.err);
