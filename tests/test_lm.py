@@ -416,6 +416,42 @@ def test_append_paged(dim, heads, kv_heads, pairs, e4m3, norm):
     clean()
 
 
+def check_cache_rows(codes, scales, y):
+    """Rows of an e4m3 cache against 64-bit heads y [rows, dim]: a head's fp32 work is within 2e-6 of its largest value, which
+    is code 448, so a code is within half a step (2^-4 of a normal code, 2^-10 of a subnormal one) and 448 * 2e-6 < 1e-3."""
+    s = scale_ref(y)
+    assert float(((scales.double() - s).abs() / s).max()) <= 3e-6
+    want = y / s[:, None]
+    assert float(((codes.double() - want).abs() - torch.clamp(want.abs() * 2.0 ** -4, min=2.0 ** -10)).max()) <= 1e-3
+
+
+@gpu
+@needs_cuda
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("pairs", ["adjacent", "halves"])
+@pytest.mark.parametrize("norm", [False, True])
+def test_append_codes_of_an_8_bit_cache(dim, pairs, norm):
+    """Every code of keys and values, heads of both sizes, channels of very different sizes."""
+    g = gen(dim)
+    heads, kv_heads, size, seqs, width = 6, 3, 16, 4, 3
+    table, pages = paged(seqs, width, seed=dim)
+    pos = torch.tensor([0, 15, 16, 47], dtype=torch.int32, device="cuda")
+    qkv = torch.randn(seqs, heads + 2 * kv_heads, dim, generator=g, device="cuda")
+    qkv = (qkv * 10.0 ** (3 * torch.rand(dim, generator=g, device="cuda") - 2)).to(BF).view(seqs, -1)
+    freqs = rope_table(width * size, dim)
+    nq, nk = (1 + 0.1 * torch.randn(dim, generator=g, device="cuda") if norm else None for _ in range(2))
+    kc, vc = (torch.zeros(pages, kv_heads, size, dim, device="cuda").to(F8) for _ in range(2))
+    ks, vs = (torch.zeros(pages, kv_heads, size, device="cuda") for _ in range(2))
+    lm_abi.append_paged(qkv, heads, kv_heads, nq, nk, 1e-6, freqs, pairs, None, pos, table, kc, vc, ks, vs)
+    x = qkv.double().view(seqs, -1, dim)
+    k, v = head_ref(x[:, heads:heads + kv_heads], nk, freqs[pos.long()], pairs), x[:, heads + kv_heads:]
+    page, slot = table[torch.arange(seqs, device="cuda"), pos.long() // size].long(), pos.long() % size
+    for cache, scale, ref in ((kc, ks, k), (vc, vs, v)):
+        got = cache.view(torch.uint8)[page, :, slot].view(F8)
+        check_cache_rows(got.reshape(-1, dim), scale[page, :, slot].reshape(-1), ref.reshape(-1, dim))
+    clean()
+
+
 @gpu
 @needs_cuda
 def test_append_reports_what_is_out_of_range():

@@ -264,6 +264,37 @@ def test_every_call_of_a_run(e4m3, monkeypatch):
 
 @gpu
 @needs_cuda
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_cache_rows_of_a_run_in_8_bits(head_dim, monkeypatch):
+    """What every append of a run leaves in an e4m3 cache, codes and scales, against the 64-bit formula on what it got."""
+    import test_lm as ops
+    from siliconed_b200 import lm, lm_abi
+    cfg = lm.DecoderConfig(dim=512, hidden=768, heads=8, kv_heads=2, head_dim=head_dim, layers=2, vocab=500, max_pos=48)
+    model = lm.Decoder(cfg, seed=5)
+    cache = lm.PagedCache(cfg, seqs=2, pages=8, page_size=16, e4m3=True)
+    real, calls = lm_abi.append_paged, []
+
+    def append(qkv, heads, kv_heads, nq, nk, eps, freqs, pairs, seq, positions, table, k, v, ks, vs):
+        q = real(qkv, heads, kv_heads, nq, nk, eps, freqs, pairs, seq, positions, table, k, v, ks, vs)
+        x = qkv.double().view(len(qkv), -1, head_dim)
+        at = positions.long()
+        page, slot = table[torch.arange(len(qkv), device="cuda"), at // 16].long(), at % 16
+        for c, s, ref in ((k, ks, ops.head_ref(x[:, heads:heads + kv_heads], nk, freqs[at], pairs, eps)), (v, vs, x[:, heads + kv_heads:])):
+            got = c.view(torch.uint8)[page, :, slot].view(torch.float8_e4m3fn)
+            ops.check_cache_rows(got.reshape(-1, head_dim), s[page, :, slot].reshape(-1), ref.reshape(-1, head_dim))
+        calls.append(len(qkv))
+        return q
+
+    monkeypatch.setattr(lm_abi, "append_paged", append)
+    seqs = [cache.admit(), cache.admit()]
+    for t in range(18):
+        model.step([t, 499 - t], seqs, cache)
+    assert calls == [2] * 18 * cfg.layers
+    assert lm_abi.errors() == (lm_abi.OK, 0)
+
+
+@gpu
+@needs_cuda
 def test_decoder_step_in_a_graph():
     from siliconed_b200 import lm_abi
     from siliconed_b200.lm import Decoder, DecoderConfig, PagedCache
