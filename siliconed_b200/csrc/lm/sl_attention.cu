@@ -531,7 +531,10 @@ __global__ void __launch_bounds__(Shape<kDim, kE4m3, kNH, kWide>::kThreads, Shap
         for (int i = 0; i < 8; ++i) x[i] = ex2(x[i] - zero[i & 1]);
         l[n][0] += (x[0] + x[2]) + (x[4] + x[6]);
         l[n][1] += (x[1] + x[3]) + (x[5] + x[7]);
-        // The one rounding to 16 bits: p (times its token's scale of v) as the MMA's operand.
+        // The one rounding to 16 bits: p (times its token's scale of v) as the MMA's operand, whose type is the cache's: f16
+        // has 11 significant bits, bf16 the 8 that the output has too (a ragged batch is 1.8e-3 from the 64-bit formula, 1.7e-3 of
+        // it the output's own rounding).  p in two bf16 terms is exact to 16 bits, but the second one may be zero or
+        // negative, and an infinity in v then becomes a NaN.
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           p[n][i >> 1][i & 1] = transpose8x8(kE4m3 ? pack_f16x2(x[2 * i] * vs[i], x[2 * i + 1] * vs[i])
