@@ -46,8 +46,11 @@ enum { SL_PAIRS_ADJACENT = 0, SL_PAIRS_HALVES = 1 };
 /*
  * z = x + delta in fp32; x_out = z rounded to x's type; y = z * rsqrt(mean(z^2) + eps) * weight; then every
  * block of 128 consecutive values of a row gets the scale s = max(max|y| / 448, 1e-30) and the codes
- * e4m3(y / s), nearest-even.  The norm sees z before it is rounded to x's type.  A block that holds a NaN or
- * an infinity has that NaN or infinity as its scale, so that all of it is NaN or infinite to a product.
+ * e4m3(y / s), nearest-even.  Both quotients are products with a reciprocal: s is within an ulp of fp32 of its
+ * definition, and what is rounded to a code within two of y / s, so that one code in many thousands, of a value
+ * that lies on the middle between two codes, is the other one of the two.  The norm sees z before it is rounded
+ * to x's type.  A block that holds a NaN or an infinity has that NaN or infinity as its scale, so that all of it
+ * is NaN or infinite to a product.
  * x, x_out [rows, d] of x_type, delta [rows, d] of delta_type (SL_BF16 or SL_F32), weight fp32 [d] (NULL: 1),
  * codes bytes [rows, d], scales fp32 [rows, ceil(d / 128)].  x_out may be x.  delta NULL: z = x, and x_out
  * must be x or NULL (nothing is written to it).  norm 0: y = z * weight, the quantization alone (eps unused).
@@ -64,8 +67,8 @@ SL_API int sl_rms_norm_quantize(const void* x, int x_type, const void* delta, in
  * q bf16 [tokens, heads, head_dim].  Token i belongs to sequence seq[i] (NULL: i) at positions[i]; its key and
  * value go to slot position % page_size of page table[seq][position / page_size], table int32
  * [seqs, table_width].  The caches are [pages, kv_heads, page_size, head_dim]: bf16, or e4m3 with fp32 scales
- * [pages, kv_heads, page_size], s = max(max|v| / 448, 1e-30) over the head's values and codes e4m3(v / s)
- * (k_scale and v_scale NULL for a bf16 cache).  A token with a negative position is padding: its q is written
+ * [pages, kv_heads, page_size], s = max(max|v| / 448, 1e-30) over the head's values and codes e4m3(v / s), its
+ * quotients as above (k_scale and v_scale NULL for a bf16 cache).  A token with a negative position is padding: its q is written
  * as zeros and nothing is appended.  head_dim 64 or 128; all tensors contiguous, 16-byte aligned.
  */
 SL_API int sl_append_paged(const uint16_t* qkv, int64_t tokens, int heads, int kv_heads, int head_dim,

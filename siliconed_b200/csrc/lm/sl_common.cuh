@@ -149,12 +149,13 @@ __device__ __forceinline__ uint32_t abs_max8(const float (&v)[8]) {
 }
 
 // The scale of values whose largest magnitude has the bits `m`: max(m / 448, 1e-30), a NaN or infinity as it is.  The
-// quotient by the constant is a product with its reciprocal (an ulp of fp32; the division would be 20 instructions).
+// quotient by the constant is a product with its reciprocal (an ulp of fp32).  With divisions here and in quantize8() the norm
+// of [4608, 3840] takes 40.4 us for 38.0, one row 3.1 for 2.6 and a prompt's append to an e4m3 cache 19.1 for 17.0.
 __device__ __forceinline__ float scale_of(uint32_t m) {
   return m >= 0x7F800000u ? __uint_as_float(m) : fmaxf(__uint_as_float(m) * (1.0f / kE4m3Max), kScaleFloor);
 }
 
-// Eight codes e4m3(v / s), by the reciprocal of s (an ulp of fp32).  s is at least 1e-30 and at most 7.6e35, so the
+// Eight codes e4m3(v / s), by the reciprocal of s (an ulp of fp32; the product's rounding makes it under two).  s is at least 1e-30 and at most 7.6e35, so the
 // reciprocal neither overflows nor is subnormal; a product past 448 by an ulp is clipped to it.
 __device__ __forceinline__ uint2 quantize8(const float (&v)[8], float s) {
   float r;
