@@ -70,6 +70,10 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// What scores are taken relative to: their maximum, but 0 where that is -inf (every p is 0 then, not NaN) or +inf (the sum is
+// +inf then, and so is its logarithm).
+__device__ __forceinline__ float zero_of(float top) { return fabsf(top) == INFINITY ? 0.0f : top; }
+
 template <bool kHalf>
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -510,7 +514,7 @@ __global__ void __launch_bounds__(Shape<kDim, kE4m3, kNH, kWide>::kThreads, Shap
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const float now = fmaxf(m[n][i], top[i]);
-          zero[i] = now == -INFINITY ? 0.0f : now;  // nothing but -inf so far: every p is 0
+          zero[i] = zero_of(now);
           top[i] = ex2(m[n][i] - zero[i]);          // the factor of what was summed before
           m[n][i] = now;
         }
@@ -626,7 +630,7 @@ __global__ void __launch_bounds__(Shape<kDim, kE4m3, kNH, kWide>::kThreads, Shap
       float top = part_m[0][r];
 #pragma unroll
       for (int w = 1; w < kWarps; ++w) top = fmaxf(top, part_m[w][r]);
-      const float zero = top == -INFINITY ? 0.0f : top;
+      const float zero = zero_of(top);
       float sum = 0.0f;
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
@@ -679,7 +683,7 @@ __global__ void __launch_bounds__(Shape<kDim, kE4m3, kNH, kWide>::kThreads, Shap
           }
 #pragma unroll
           for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
-          const float zero = top == -INFINITY ? 0.0f : top;
+          const float zero = zero_of(top);
           float sum = 0.0f;
           for (int w = lane; w < count; w += 32) {
             const float2 ml = factor[r * count + w];

@@ -687,6 +687,54 @@ def test_attention_extremes():
 
 @gpu
 @needs_cuda
+@pytest.mark.parametrize("n", [1, 20, 3000, 40000])
+def test_scores_that_are_all_minus_infinity(n):
+    """Zeros and lse -inf, in one warp's step and over a context cut between CTAs."""
+    dim, size = 128, 16
+    width = -(-n // size)
+    table = torch.arange(width, dtype=torch.int32, device="cuda").view(1, -1)
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    kc, vc = (torch.randn(width, 1, size, dim, generator=gen(n), device="cuda").to(BF) for _ in range(2))
+    kc[..., 7] = -math.inf
+    q = torch.ones(1, 2, dim, dtype=BF, device="cuda")
+    lse = torch.empty(1, 2, device="cuda")
+    out = lm_abi.paged_attention(q, kc, vc, None, None, table, lens, 0.05, lse=lse)
+    assert not out.any() and bool((lse == -math.inf).all())
+    clean()
+
+
+@gpu
+@needs_cuda
+@pytest.mark.parametrize("n", [1, 20, 3000, 40000])
+def test_a_score_of_infinity(n):
+    """+inf among finite scores: what the formula gives, lse +inf and inf / inf = NaN.  -inf for the other head: left out."""
+    g = gen(n)
+    dim, size = 128, 16
+    width = -(-n // size)
+    table = torch.arange(width, dtype=torch.int32, device="cuda").view(1, -1)
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    kc, vc = (torch.randn(width, 1, size, dim, generator=g, device="cuda").to(BF) for _ in range(2))
+    q = torch.randn(1, 2, dim, generator=g, device="cuda").to(BF)
+    q[0, 0, 0], q[0, 1, 0] = 1, -1
+    kc[(n // 2) // size, 0, (n // 2) % size, 0] = math.inf
+    lse = torch.empty(1, 2, device="cuda")
+    out = lm_abi.paged_attention(q, kc, vc, None, None, table, lens, 0.05, lse=lse)
+    assert bool(out[0, 0].isnan().all()) and float(lse[0, 0]) == math.inf
+    keep = [i for i in range(n) if i != n // 2]
+    if not keep:
+        assert not out[0, 1].any() and float(lse[0, 1]) == -math.inf
+    else:
+        kk, vv = (rows_of(c, None, table, 0, n, 0)[keep] for c in (kc, vc))
+        s = q[0, 1:].double() @ kk.t() * 0.05
+        p = torch.softmax(s, -1)
+        ref, mass = p @ vv, p @ vv.abs()
+        assert float(((out[0, 1:].double() - ref).abs() / (U * 1.01 * (mass + ref.abs()) + 4e-5 * mass)).max()) <= 1
+        assert float((lse[0, 1:].double() - torch.logsumexp(s, -1)).abs().max()) <= 1e-4
+    clean()
+
+
+@gpu
+@needs_cuda
 def test_cache_beyond_four_gigabytes():
     dim, size, kv_heads = 128, 64, 8
     pages = (5 << 30) // (size * kv_heads * dim * 2)
