@@ -172,17 +172,16 @@ struct Shape {
   static constexpr int kSmem = kWarps * kWarpBytes;
   static constexpr int kPartRow = kDim + 4;
   static constexpr int kPartFloats = kRows * (kDim + 2);
-  // A launch's shared memory on `workers` CTAs.  The ring also holds the factors of a cut context's parts when they are
-  // added, 8 bytes a row and part, and one context may be cut over every CTA: what the four-warp shapes' rings of 32 to 35 KB
-  // do not hold (592 parts of 8 rows: 37 KB).
+  // A launch's shared memory on `workers` CTAs.  The ring also holds the factors of a cut context's parts when they are added,
+  // a float a row and part, and one context may be cut over every CTA.  (Two floats: 592 parts of 8 rows pass the four-warp
+  // shapes' rings of 32 to 35 KB, and the 3 KB more take so much of the L1 that 64 ragged e4m3 contexts are 1.7 % slower.)
   static constexpr int smem_bytes(int workers) {
-    const int factors = kRows * workers * static_cast<int>(sizeof(float2));
+    const int factors = kRows * workers * static_cast<int>(sizeof(float));
     return factors > kSmem ? factors : kSmem;
   }
   static_assert(kRows * kPartRow * 4 <= kWarpBytes, "the join's part fits the ring");
   static_assert(!kE4m3 || kSlots % 2 == 0, "the scales go with whole steps");
-  // 6 KB a CTA beside the ring: the lengths, the first units, the joins' statistics and what the device keeps.
-  static_assert((smem_bytes(148 * kCtasPerSm) + 6 * 1024) * kCtasPerSm <= 227 * 1024, "a B200's SM holds its CTAs");
+  static_assert(smem_bytes(148 * kCtasPerSm) == kSmem, "a B200's rings hold the factors of as many parts as there are CTAs");
 };
 constexpr int kMostCtasPerSm = 4;
 
@@ -673,24 +672,22 @@ __global__ void __launch_bounds__(Shape<kDim, kE4m3, kNH, kWide>::kThreads, Shap
 #pragma unroll
         for (int w = 0; w < kEarly; ++w)
           if (w < count && tid / kRun < rows) early[w] = __ldcg(reinterpret_cast<const float4*>(part_of(w) + tid / kRun * kDim + d0));
-        float2* factor = reinterpret_cast<float2*>(ring);  // [rows][count]: m, then exp(m - top), and l; see smem_bytes()
+        float* factor = reinterpret_cast<float*>(ring);  // [rows][count]: m, then exp(m - top); see smem_bytes()
         for (int r = warp; r < rows; r += kWarps) {
-          float top = -INFINITY;
+          float mine = -INFINITY, sum = 0.0f;  // of this lane's parts
           for (int w = lane; w < count; w += 32) {
             const float2 ml = __ldcg(reinterpret_cast<const float2*>(part_of(w) + kRows * kDim + 2 * r));
-            factor[r * count + w] = ml;
-            top = fmaxf(top, ml.x);
+            factor[r * count + w] = ml.x;
+            const float now = fmaxf(mine, ml.x), from = zero_of(now);
+            sum = sum * ex2(mine - from) + ml.y * ex2(ml.x - from);
+            mine = now;
           }
+          float top = mine;
 #pragma unroll
           for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
           const float zero = zero_of(top);
-          float sum = 0.0f;
-          for (int w = lane; w < count; w += 32) {
-            const float2 ml = factor[r * count + w];
-            const float f = ex2(ml.x - zero);
-            factor[r * count + w].x = f;
-            sum += f * ml.y;
-          }
+          sum *= ex2(mine - zero);
+          for (int w = lane; w < count; w += 32) factor[r * count + w] = ex2(factor[r * count + w] - zero);
 #pragma unroll
           for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, off);
           if (lane == 0) {
@@ -702,7 +699,7 @@ __global__ void __launch_bounds__(Shape<kDim, kE4m3, kNH, kWide>::kThreads, Shap
         for (int r = tid / kRun; r < rows; r += kRowStep) {
           float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
           const auto add = [&](float4 v, int w) {
-            const float f = factor[r * count + w].x;
+            const float f = factor[r * count + w];
             acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
           };
           if (r == tid / kRun) {
