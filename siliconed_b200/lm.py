@@ -18,6 +18,12 @@ from .lm_abi import BLOCK, LmError
 E4M3_MAX = 448.0
 
 
+def _device(device) -> torch.device:
+    """The device with its index: a bare "cuda" is another one whenever the current device changes."""
+    device = torch.device("cuda") if device is None else torch.device(device)
+    return torch.device("cuda", torch.cuda.current_device()) if device.type == "cuda" and device.index is None else device
+
+
 @dataclass
 class DecoderConfig:
     """The defaults are the widths of the text encoder whose int8 shapes the encoder prefill workload uses."""
@@ -67,7 +73,7 @@ class PagedCache:
     """
 
     def __init__(self, cfg: DecoderConfig, seqs: int, pages: int, page_size: int = 16, e4m3: bool = False, device=None):
-        device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        device = _device(device)
         shape = (cfg.layers, pages, cfg.kv_heads, page_size, cfg.head_dim)
         kind = torch.float8_e4m3fn if e4m3 else torch.bfloat16
         self.k, self.v = (torch.zeros(shape, dtype=kind, device=device) for _ in range(2))
@@ -152,7 +158,8 @@ class DecoderLayer:
         self.down = weight(cfg.dim, cfg.hidden)
 
     def forward(self, x, delta, freqs, positions, table, lengths, cache, workspace=None):
-        """One new token per sequence: x fp32 [batch, dim] += delta in place; returns the layer's own addition (bf16)."""
+        """One new token per sequence: x fp32 [batch, dim] += delta in place; returns the layer's own addition (bf16).  The
+        tensors' device is the current one (the activation runs on the current device's stream)."""
         cfg = self.cfg
         batch = x.shape[0]
         _, codes, scales = lm_abi.rms_norm_quantize(x, delta, self.norm1, cfg.eps)
@@ -171,7 +178,7 @@ class Decoder:
     """Embedding, layers and logits with random weights of a seed; ``step`` decodes one token for each given sequence."""
 
     def __init__(self, cfg: DecoderConfig, seed: int = 0, device=None):
-        device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        device = _device(device)
         g = torch.Generator(device=device).manual_seed(seed)
         self.cfg, self.device = cfg, device
         self.embedding = torch.randn(cfg.vocab, cfg.dim, generator=g, device=device)
@@ -184,11 +191,12 @@ class Decoder:
         """Logits fp32 [batch, vocab] of tokens int64 [batch], each below vocab (not checked here: they are on the device), at
         positions int32 [batch]; table int32 [batch, width] and lengths int32 [batch] (the new tokens counted) are the
         sequences' rows."""
-        x, delta = self.embedding[tokens], None
-        for i, layer in enumerate(self.layers):
-            delta = layer.forward(x, delta, self.freqs, positions, table, lengths, cache.layer(i), workspace)
-        _, codes, scales = lm_abi.rms_norm_quantize(x, delta, self.norm, self.cfg.eps)
-        return self.head(codes, scales, torch.empty(x.shape[0], self.cfg.vocab, device=self.device))
+        with torch.cuda.device(self.device):
+            x, delta = self.embedding[tokens], None
+            for i, layer in enumerate(self.layers):
+                delta = layer.forward(x, delta, self.freqs, positions, table, lengths, cache.layer(i), workspace)
+            _, codes, scales = lm_abi.rms_norm_quantize(x, delta, self.norm, self.cfg.eps)
+            return self.head(codes, scales, torch.empty(x.shape[0], self.cfg.vocab, device=x.device))
 
     def step(self, tokens: list[int], seqs: list[int], cache: PagedCache):
         """Appends one token to each sequence and returns its logits."""

@@ -94,6 +94,34 @@ def test_step_refuses_tokens_that_the_embedding_does_not_have():
     assert cache.lengths == [0, 0] and len(cache._free) == 8
 
 
+def test_forward_runs_on_the_models_device(monkeypatch):
+    """The activation between the products goes to the current device's stream: it has to be the model's device."""
+    import contextlib
+    from siliconed_b200 import lm
+    entered, seen = [], []
+
+    @contextlib.contextmanager
+    def guard(device):
+        entered.append(device)
+        yield
+        entered.pop()
+
+    class Layer:
+        def forward(self, *args):
+            seen.append(list(entered))
+
+    monkeypatch.setattr(torch.cuda, "device", guard)
+    monkeypatch.setattr(lm.lm_abi, "rms_norm_quantize", lambda *a: (seen.append(list(entered)), None, None))
+    model = lm.Decoder.__new__(lm.Decoder)
+    model.cfg = lm.DecoderConfig(dim=4, layers=2, vocab=3)
+    model.device, model.layers, model.embedding = torch.device("cuda", 1), [Layer(), Layer()], torch.zeros(3, 4)
+    model.freqs = model.norm = None
+    model.head = lambda codes, scales, out: out
+    cache = lm.PagedCache(lm.DecoderConfig(layers=2, max_pos=16, kv_heads=1), seqs=1, pages=1, device="cpu")
+    out = model.forward(torch.tensor([1, 2]), None, None, None, cache)
+    assert out.shape == (2, 3) and seen == [[model.device]] * 3 and not entered
+
+
 def test_step_of_no_sequences():
     from siliconed_b200.lm import Decoder, DecoderConfig, PagedCache
     cfg = DecoderConfig(dim=256, hidden=512, heads=2, kv_heads=1, layers=1, vocab=300, max_pos=64)
