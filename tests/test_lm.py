@@ -902,3 +902,23 @@ def test_linear_keeps_scales_apart_and_nan_in_its_row(m):
     assert bool(y[1].isnan().all()) and int(y.isnan().any(1).sum()) == 1
     assert lm_abi.linear_block_fp8(codes[:0], scales[:0], w, ws).shape == (0, n)
     clean()
+
+
+@gpu
+@needs_cuda
+@pytest.mark.parametrize("m,n,k", [(1500, 2560, 1024), (1501, 2567, 1040), (500, 2560, 5040)])
+def test_many_rows_keep_scales_apart_and_nan_in_its_row(m, n, k):
+    """The same of the kernel of CTA pairs: whole tiles, rows that start on any value, K shared by several pairs."""
+    g = gen(m + k)
+    kb, nb = -(-k // 128), -(-n // 128)
+    codes = torch.randn(m, k, generator=g, device="cuda").to(F8)
+    scales = 10.0 ** torch.randint(-6, 7, (m, kb), generator=g, device="cuda").float()
+    w = torch.randn(n, k, generator=g, device="cuda").to(F8)
+    ws = 10.0 ** torch.randint(-6, 7, (nb, kb), generator=g, device="cuda").float()
+    y = lm_abi.linear_block_fp8(codes, scales, w, ws, None, torch.empty(m, n, device="cuda"))
+    check_product(codes, scales, w, ws, None, y)
+    scales[257, kb - 1] = math.nan
+    for dtype in (BF, torch.float32):
+        y = lm_abi.linear_block_fp8(codes, scales, w, ws, None, torch.empty(m, n, dtype=dtype, device="cuda"))
+        assert bool(y[257].isnan().all()) and int(y.isnan().any(1).sum()) == 1
+    clean()
