@@ -739,7 +739,8 @@ cudaError_t launch_attention(const Attention& a, int sms, cudaStream_t stream) {
 
 template <int kDim, bool kE4m3>
 cudaError_t launch_kind(const Attention& a, int sms, cudaStream_t stream) {
-  // Four-warp CTAs cut a long context into so many parts (444 over few contexts) that adding them costs more than the
+  // By the table's room, since the host does not know the lengths: few short contexts in a table for long ones take the wide
+  // form.  Four-warp CTAs cut a long context into so many parts (444 over few contexts) that adding them costs more than the
   // switches between contexts that they hide: 4 contexts of 131072 tokens 87 us, wide 68; but 8 of 16 tokens 4.9, wide
   // 7.7, and 2048 of 128 tokens 42 either way (B200, heads of 128).
   const bool wide = static_cast<int64_t>(a.batch) * a.kv_heads * a.subs < 64 &&

@@ -13,8 +13,8 @@
 //   memory by TMA stores, which run under the next tile's blocks.  What bounds it is a block's round trip through its TMEM
 //   buffer: 4 MMAs (650 cycles beside the epilogue's work), their commit (350), the partial read by 16 warps (450) and the
 //   buffer's release to the MMA threads (400), some 1900 cycles for the two buffers that 256 columns leave.  [4096, 3840] x
-//   [3840, 10240]: 182 us, 1770 TFLOP/s (191 to 205 with inputs that change from call to call); without the epilogue's
-//   arithmetic 134 us, the loads take less.  (Beside the 182: tiles of 256 x 128 with four buffers 198 us, their MMAs read
+//   [3840, 10240]: 172 us, 1870 TFLOP/s in a chain of calls (191 to 205 with new inputs in every call); without the epilogue's
+//   arithmetic 134 us, the loads take less.  (Beside an earlier form's 182: tiles of 256 x 128 with four buffers 198 us, their MMAs read
 //   shared memory half again as often; fma.rn.f32x2 for the sums 293, pairs of registers moved together; one issuing
 //   thread 212; the two halves of the columns issued by a thread each, two buffers each, 5 % slower, a is read twice; 16
 //   epilogue warps of 64 columns 258, spills.)  Where the tiles leave pairs idle, a cluster of up to 4 pairs shares a
@@ -23,9 +23,11 @@
 //   M and the rows of a, in tiles of up to 64, its N, so that no MMA row or TMEM column is padding; K is cut over the
 //   CTAs of a cluster, whose partials meet through distributed shared memory and are added in rank order.  The weight's
 //   first tiles are prefetched to L2 while the kernel before this one ends.  One row of [4096, 12288] (from HBM, calls after
-//   one another): 12.0 us, 4.2 TB/s (0.65 of a copy's rate); 64 rows of it 17.0 us, 131 rows of [2560, 9728] 12.9 us, bound
-//   by the epilogue's instructions and by shared memory, which the copies, the MMAs' operands and the factors keep busy for some
-//   400 cycles a block of 64 rows; eight epilogue warps spill and are slower.  (Room for a third
+//   one another): 12.1 us, 4.2 TB/s (0.65 of a copy's rate): its begin, the cluster's join and its end take some 4 us, and 192
+//   equal CTAs on 148 SMs leave 44 SMs with twice the others' bytes.  64 rows of it 17.0 us, 131 rows of [2560, 9728] 12.9 us:
+//   the weight passes through shared memory once for each tile of rows, three times, 228 equal CTAs lie unevenly on the SMs, and
+//   a block's chain of commit, TMEM read and sums in four warps is waited for; no resource is full (issue slots 35 %, tensor
+//   pipe 12 %).  Eight epilogue warps spill and are slower.  (Room for a third
 //   CTA an SM, so that the next call's begin early: 15.4 us for one row, the CTAs spread unevenly.)
 //
 // Rows past m or n and values past k arrive as zeros.  Every wait is bounded; no load uses cluster multicast.
@@ -307,7 +309,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       } else {
         // Rows that do not start on 16 bytes: through shared memory all the same, so that a warp's stores are of neighbours.
-        // (Every lane along its own row: 178 us for [2000, 9728] x [9728, 2567], this way 98; 94 for 2560 columns.)
+        // (Every lane along its own row: 178 us for [2000, 9728] x [9728, 2567], this way 94; 88 for 2560 columns.)
         constexpr int kPassCols = kF32Out ? 64 : 128, kPer = kF32Out ? 4 : 8;  // 256 bytes of a row; values of 16 bytes
         uint8_t* out = &s.out[ew][0][0];
         const int rows = min(32, m - row0);
@@ -873,7 +875,8 @@ int cluster_capacity(int c, int dev) {
 
 // Estimated microseconds with the weight in HBM, fitted (B200) to [m, 4096] x [4096, 12288 or 4096], [m, 12288] x [12288, 4096],
 // [m, 2560] x [2560, 9728 or 2560], [m, 9728] x [9728, 2560] and [m, 512] x [512, 1000], m 1 to 1024 and 1 to 8 parts; most
-// within 10 %.  The few-rows kernel: a begin and an end, longer where a cluster adds (and then for every wave); a CTA's
+// within 10 %.  None of these has a long output and a short K, and neither estimate has a term for the output's bytes: [1000, 1024]
+// x [1024, 7001] is estimated at 16 us and takes 25 (4.3 by its bytes and operations).  The few-rows kernel: a begin and an end, longer where a cluster adds (and then for every wave); a CTA's
 // blocks one after another, slower with more rows and more CTAs an SM, so that a last wave of few CTAs is shorter; and the
 // weight's bytes.  The parts this picks are the fastest or within 3 % of them.
 struct SwapPlan {
