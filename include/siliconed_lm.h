@@ -68,8 +68,9 @@ SL_API int sl_rms_norm_quantize(const void* x, int x_type, const void* delta, in
  * value go to slot position % page_size of page table[seq][position / page_size], table int32
  * [seqs, table_width].  The caches are [pages, kv_heads, page_size, head_dim]: bf16, or e4m3 with fp32 scales
  * [pages, kv_heads, page_size], s = max(max|v| / 448, 1e-30) over the head's values and codes e4m3(v / s), its
- * quotients as above (k_scale and v_scale NULL for a bf16 cache).  A token with a negative position is padding: its q is written
- * as zeros and nothing is appended.  head_dim 64 or 128; all tensors contiguous, 16-byte aligned.
+ * quotients as above (k_scale and v_scale NULL for a bf16 cache).  A token with a negative position is padding: its
+ * q is written as zeros and nothing is appended; so is that of a position past max_pos, which is reported.  No two
+ * tokens of a call share a slot.  head_dim 64 or 128; all tensors contiguous, 16-byte aligned.
  */
 SL_API int sl_append_paged(const uint16_t* qkv, int64_t tokens, int heads, int kv_heads, int head_dim,
                            const float* norm_q, const float* norm_k, float eps, const float* freqs, int max_pos,

@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(kThreads, kResident<kDim, kE4m3>) append_paged
     for (int t = 0; t < 8; ++t) ss += v[0][t] * v[0][t] + v[1][t] * v[1][t];
 #pragma unroll
     for (int off = kLanes / 2; off > 0; off >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, off);
-    if (!is_v) {
+    if (!is_v && pos >= 0) {  // padding stays zeros, whatever eps and the rotation table's first row are
       if (norm != nullptr) {
         const float inv = rsqrtf(ss * (1.0f / kDim) + a.eps);
 #pragma unroll

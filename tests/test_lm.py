@@ -416,6 +416,30 @@ def test_append_paged(dim, heads, kv_heads, pairs, e4m3, norm):
     clean()
 
 
+@gpu
+@needs_cuda
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("pairs", ["adjacent", "halves"])
+def test_append_writes_zeros_for_padding(dim, pairs):
+    """Whatever there is to be multiplied with: eps 0 (0 * rsqrt(0) is NaN), NaN in the padded rows, in the rotation table's
+    first row, for padding and for positions past the table."""
+    size = 16
+    table = torch.tensor([[0, 1]], dtype=torch.int32, device="cuda")
+    qkv = torch.ones(3, 4 * dim, dtype=BF, device="cuda")
+    qkv[1:] = math.nan
+    freqs = rope_table(20, dim)
+    freqs[0] = math.nan
+    norm = torch.ones(dim, device="cuda")
+    kc, vc = (torch.zeros(2, 1, size, dim, dtype=BF, device="cuda") for _ in range(2))
+    seq = torch.zeros(3, dtype=torch.int32, device="cuda")
+    pos = torch.tensor([5, -1, 20], dtype=torch.int32, device="cuda")
+    q = lm_abi.append_paged(qkv, 2, 1, norm, norm, 0.0, freqs, pairs, seq, pos, table, kc, vc)
+    assert lm_abi.errors()[0] == lm_abi.OUT_OF_RANGE  # position 20
+    assert not q[1:].any() and bool(q[0].isfinite().all())
+    assert int(vc.any(-1).sum()) == 1 and int(kc.any(-1).sum()) == 1
+    clean()
+
+
 def check_cache_rows(codes, scales, y):
     """Rows of an e4m3 cache against 64-bit heads y [rows, dim]: a head's fp32 work is within 2e-6 of its largest value, which
     is code 448, so a code is within half a step (2^-4 of a normal code, 2^-10 of a subnormal one) and 448 * 2e-6 < 1e-3."""
