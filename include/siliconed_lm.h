@@ -84,9 +84,10 @@ SL_API int sl_append_paged(const uint16_t* qkv, int64_t tokens, int heads, int k
  * h reads key-value head h / (heads / kv_heads).  q, out bf16 [batch, heads, head_dim]; lse fp32 [batch,
  * heads] (NULL: not wanted) gets log sum_t exp(scale q . k_t).  A sequence of length 0 (or whose scores are
  * all -inf, with finite values) gives zeros and lse -inf; a score of +inf gives NaN and lse +inf.  Slots past a
- * sequence's length are not read.  Scores, softmax statistics and sums are fp32.  For the product with v, p is
- * rounded to bf16; with an e4m3 cache p times its token's scale of v to f16, relative to the largest such scale of
- * the context so far: a term below 2^-29 of that scale has fewer than f16's 11 bits, one below 2^-40 none.
+ * sequence's length are not read.  Scores, softmax statistics and sums are fp32.  For the product with v, p is held
+ * to 16 bits (two bf16 terms); with an e4m3 cache p times its token's scale of v is rounded to f16, relative to the
+ * largest such scale of the context so far: a term below 2^-29 of that scale has fewer than f16's 11 bits, one below
+ * 2^-40 none.
  * head_dim 64 or 128; kv_heads divides heads.  The workspace (sl_paged_attention_workspace bytes, 16-byte
  * aligned) must be zero before its first use; every call leaves it ready for the next one.  Calls that may run
  * at the same time need workspaces of their own.

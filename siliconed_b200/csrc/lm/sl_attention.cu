@@ -494,7 +494,10 @@ __global__ void __launch_bounds__(Shape<kDim, kE4m3, kNH, kWide>::kThreads, Shap
 #pragma unroll
         for (int i = 0; i < 4; ++i) vs[i] *= f;
       }
-      uint32_t p[kNH][2][2];  // P^T as the B operand: head g, tokens 2 c, 2 c + 1 and 2 c + 8, 2 c + 9 of each tile
+      // P^T as the B operand: head g, tokens 2 c, 2 c + 1 and 2 c + 8, 2 c + 9 of each tile.
+      constexpr int kTerms = kE4m3 ? 1 : 2;
+      constexpr float kTiny = 1.1754944e-38f;
+      uint32_t p[kTerms][kNH][2][2];
 #pragma unroll
       for (int n = 0; n < kNH; ++n) {
         float x[8];  // tokens g + 8 (i >> 1), query head 2 c + (i & 1)
@@ -534,14 +537,22 @@ __global__ void __launch_bounds__(Shape<kDim, kE4m3, kNH, kWide>::kThreads, Shap
         for (int i = 0; i < 8; ++i) x[i] = ex2(x[i] - zero[i & 1]);
         l[n][0] += (x[0] + x[2]) + (x[4] + x[6]);
         l[n][1] += (x[1] + x[3]) + (x[5] + x[7]);
-        // The one rounding to 16 bits: p (times its token's scale of v) as the MMA's operand, whose type is the cache's: f16
-        // has 11 significant bits, bf16 the 8 that the output has too (a ragged batch is 1.8e-3 from the 64-bit formula, 1.7e-3 of
-        // it the output's own rounding).  p in two bf16 terms is exact to 16 bits, but the second one may be zero or
-        // negative, and an infinity in v then becomes a NaN.
+        // The one rounding to 16 bits, to be the MMA's operand, whose type is the cache's.  f16: p times its token's scale of v, 11
+        // significant bits.  bf16: p in two terms, its upper 8 bits and the next 8 (in one term of 8 its error would stand
+        // beside the output's own; the second one costs 33 ragged contexts 0.3 %, one long one 0.8 %, up to 5 % where 16 query heads
+        // share a key-value head).  It is at least the smallest normal number where p is not 0: an infinity in v times it is that
+        // infinity again, not NaN.
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          p[n][i >> 1][i & 1] = transpose8x8(kE4m3 ? pack_f16x2(x[2 * i] * vs[i], x[2 * i + 1] * vs[i])
-                                                   : pack_bf16x2(x[2 * i], x[2 * i + 1]));
+        for (int i = 0; i < 4; ++i) {
+          const float a = x[2 * i], b = x[2 * i + 1];
+          const uint32_t upper = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+          p[0][n][i >> 1][i & 1] = transpose8x8(kE4m3 ? pack_f16x2(a * vs[i], b * vs[i]) : upper);
+          if (!kE4m3) {
+            const float rest_a = fmaxf(a - __uint_as_float(__float_as_uint(a) & 0xFFFF0000u), fminf(a, kTiny));
+            const float rest_b = fmaxf(b - __uint_as_float(__float_as_uint(b) & 0xFFFF0000u), fminf(b, kTiny));
+            p[kTerms - 1][n][i >> 1][i & 1] = transpose8x8(pack_bf16x2(rest_a, rest_b));
+          }
+        }
       }
       const uint8_t* const values = arrival();
       if ((gave_up = values == nullptr)) break;
@@ -572,14 +583,16 @@ __global__ void __launch_bounds__(Shape<kDim, kE4m3, kNH, kWide>::kThreads, Shap
                 e4m3x4_to_f16(__byte_perm(v[2][w], v[3][w], half == 0 ? 0x5140 : 0x7362), a2, a3);
 #pragma unroll
                 for (int n = 0; n < kNH; ++n)
-                  mma16816<true>(o[n][e * (kVDims / 2) + 2 * w + half], a0, a1, a2, a3, p[n][t][0], p[n][t][1]);
+                  mma16816<true>(o[n][e * (kVDims / 2) + 2 * w + half], a0, a1, a2, a3, p[0][n][t][0], p[0][n][t][1]);
               }
             } else {
               const uint32_t a0 = __byte_perm(v[0][w], v[1][w], 0x5410), a1 = __byte_perm(v[0][w], v[1][w], 0x7632);
               const uint32_t a2 = __byte_perm(v[2][w], v[3][w], 0x5410), a3 = __byte_perm(v[2][w], v[3][w], 0x7632);
 #pragma unroll
               for (int n = 0; n < kNH; ++n)
-                mma16816<false>(o[n][e * (kVDims / 2) + w], a0, a1, a2, a3, p[n][t][0], p[n][t][1]);
+#pragma unroll
+                for (int term = 0; term < kTerms; ++term)
+                  mma16816<false>(o[n][e * (kVDims / 2) + w], a0, a1, a2, a3, p[term][n][t][0], p[term][n][t][1]);
             }
           }
         }

@@ -711,6 +711,51 @@ def test_attention_extremes():
 
 @gpu
 @needs_cuda
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("dim,heads,kv_heads", [(128, 8, 2), (64, 8, 2), (128, 32, 2), (64, 32, 2)])
+def test_attention_loses_no_more_than_its_output_rounding(dim, heads, kv_heads, e4m3):
+    """p's own rounding on the way to the product with v: upper 8 bits and the rest rounded to 8 (2^-7 2^-8 of p at most) over a
+    bf16 cache, f16 (2^-11, twice as much for the scale's product) over an e4m3 one.  Values that nearly cancel show it."""
+    g = gen(dim + heads)
+    lengths = [2, 3, 5, 40, 700]
+    table, pages = paged(len(lengths), 45)
+    k, v = make_cache(g, pages, kv_heads, 16, dim, e4m3)
+    q = (torch.randn(len(lengths), heads, dim, generator=g, device="cuda") * 2).to(BF)
+    lens = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    out = lm_abi.paged_attention(q, k[0], v[0], k[1], v[1], table, lens, 1 / math.sqrt(dim))
+    for b, n in enumerate(lengths):
+        for h in range(kv_heads):
+            of = slice(h * heads // kv_heads, (h + 1) * heads // kv_heads)
+            kk, vv = rows_of(*k, table, b, n, h), rows_of(*v, table, b, n, h)
+            p = torch.softmax(q[b, of].double() @ kk.t() / math.sqrt(dim), -1)
+            ref, mass = p @ vv, p @ vv.abs()
+            room = U * 1.01 * ref.abs() + (4e-5 + (2.0 ** -10 if e4m3 else 2.0 ** -15)) * mass
+            assert float(((out[b, of].double() - ref).abs() / room).max()) <= 1, (b, n, h)
+    clean()
+
+
+@gpu
+@needs_cuda
+def test_infinite_values_stay_infinite():
+    """Whatever p is: 1, a power of two, all of its bits set, tiny."""
+    dim, size = 128, 16
+    q = torch.zeros(1, 1, dim, dtype=BF, device="cuda")
+    q[..., 0] = 1
+    table = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    lens = torch.tensor([4], dtype=torch.int32, device="cuda")
+    for far in (0.0, -1.0, -0.3, -7.7, -60.0):  # the second token's score below the first one's
+        kc, vc = (torch.zeros(1, 1, size, dim, dtype=BF, device="cuda") for _ in range(2))
+        kc[0, 0, :, 0] = 3
+        kc[0, 0, 1, 0] = 3 + far
+        vc[0, 0, 1, 3], vc[0, 0, 1, 4], vc[0, 0, 2, 5], vc[0, 0, 3, 6] = math.inf, -math.inf, math.inf, -math.inf
+        out = lm_abi.paged_attention(q, kc, vc, None, None, table, lens, 1.0)[0, 0]
+        assert [float(out[i]) for i in (3, 4, 5, 6)] == [math.inf, -math.inf, math.inf, -math.inf], far
+        assert not out[:3].any() and not out[7:].any()
+    clean()
+
+
+@gpu
+@needs_cuda
 @pytest.mark.parametrize("n", [1, 20, 3000, 40000])
 def test_scores_that_are_all_minus_infinity(n):
     """Zeros and lse -inf, in one warp's step and over a context cut between CTAs."""
