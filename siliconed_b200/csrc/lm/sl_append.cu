@@ -4,7 +4,7 @@
 //
 // Bound by latency: for single tokens a launch's, for prompts that of the dependent reads with which every CTA begins (the
 // position, then the sequence and page, and the (cos, sin) of that position), three rounds of CTAs one after another for 2711
-// tokens: issue slots are taken in 55 % of the cycles and waiting for loads is the first stall; 17 us where the bytes take 8.6.
+// tokens: issue slots are taken in 54 % of the cycles and waiting for loads is the first stall; 17 us where the bytes take 8.6.
 // One CTA per token;
 // groups of head_dim / 16 lanes take its heads in turns, three turns' loads at once, with the token's (cos, sin) and page
 // slot loaded once.  A lane holds 8 values of a head's first half and the same 8 of its second half, so both orders of
